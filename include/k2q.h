@@ -147,6 +147,39 @@ int k2q_sigmoid_gate_bwd(const void* dy, int64_t lddy, const void* a, int64_t ld
 int k2q_gate_residual(const void* x_or_null, int64_t ldx, const void* y, int64_t ldy, const void* gate_bk,
                       int64_t rows_per_batch, int64_t M, int64_t K, void* out, int64_t ldo, void* stream);
 
+/* ---- residual update + RMS norm + modulation as one step (mmdit.py:310-321, 237-246) --------------------
+ *   stream = bf16(x + gate_b * y)   (gate NULL: x + y)
+ *   h      = stream * rstd * (1 + norm_scale) * (1 + mod_scale_b) + mod_shift_b,   rstd = (mean stream^2 + eps)^-1/2
+ * with b = row / rows_per_batch (M a multiple of it), gate / mod_scale / mod_shift [B, K] bf16, each or NULL.
+ * Unlike the single steps above, which round to bf16 where the reference's eager code does, everything
+ * between the loads and the stores is fp32; the norm reads the stream as it is kept (bf16).  Row strides are
+ * multiples of 8 elements, bases 16-byte aligned, K <= 16384.
+ *   quant  K a multiple of 128: h rotated and quantised like k2q_fwht_quant_act_i8 (xq [M, K], sx [M]); stream
+ *          may be x itself (same pointer and stride) or y itself, but must not overlap them otherwise
+ *   fwd    K a multiple of 8: dense h [M, ldh] and rstd [M]; the same rule for stream; h overlaps nothing
+ *   bwd    from dstream, dh (either NULL: zero), the kept stream, rstd:  n = stream * rstd,
+ *          g = dh (1 + norm_scale)(1 + mod_scale_b),  d = dstream + rstd (g - n mean(g n))
+ *          dx = d, dy = gate_b * d (either NULL: not wanted); where the pointers are given, sums over a
+ *          sample's rows: dgate [B, K] = sum d y (needs y), dmod_scale = (1 + norm_scale) sum dh n,
+ *          dmod_shift = sum dh (bf16), and dnorm [K] f32 = sum_b (1 + mod_scale_b) sum dh n.  The sums are formed in
+ *          fp32 in a fixed order in a workspace of k2q_residual_norm_bwd_workspace_bytes() bytes (16-byte aligned;
+ *          may be NULL when no sum is wanted).                                                            */
+int k2q_residual_norm_quant(const void* x_bf16, int64_t ldx, const void* y_bf16, int64_t ldy, const void* gate_bf16,
+                            const float* norm_scale, const void* mod_scale_bf16, const void* mod_shift_bf16,
+                            int64_t rows_per_batch, int64_t M, int64_t K, float eps, void* stream_bf16, int64_t lds,
+                            int8_t* xq, float* sx, void* stream);
+int k2q_residual_norm_fwd(const void* x_bf16, int64_t ldx, const void* y_bf16, int64_t ldy, const void* gate_bf16,
+                          const float* norm_scale, const void* mod_scale_bf16, const void* mod_shift_bf16,
+                          int64_t rows_per_batch, int64_t M, int64_t K, float eps, void* stream_bf16, int64_t lds,
+                          void* h_bf16, int64_t ldh, float* rstd, void* stream);
+int64_t k2q_residual_norm_bwd_workspace_bytes(int64_t rows_per_batch, int64_t M, int64_t K);
+int k2q_residual_norm_bwd(const void* dstream_bf16, int64_t ldds, const void* dh_bf16, int64_t lddh,
+                          const void* stream_bf16, int64_t lds, const float* rstd, const void* y_bf16, int64_t ldy,
+                          const void* gate_bf16, const float* norm_scale, const void* mod_scale_bf16,
+                          int64_t rows_per_batch, int64_t M, int64_t K, void* dx_bf16, int64_t lddx, void* dy_bf16,
+                          int64_t lddy, void* dgate_bf16, void* dmod_scale_bf16, void* dmod_shift_bf16, float* dnorm,
+                          void* ws, int64_t ws_bytes, void* stream);
+
 /* Per-token int8 quantisation WITHOUT rotation of g[m,n] * colscale[n] (colscale may be
  * NULL).  Used by the backward (autograd of quantize.py:51): dY is folded with the
  * per-out-channel weight scale, which sits on the contraction index of dX = dY.W.      */

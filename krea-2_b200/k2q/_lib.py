@@ -74,6 +74,12 @@ SIGNATURES = {
     "k2q_sigmoid_gate_fwd": (C.c_int, [_p, _i64, _p, _i64, _i64, _i64, _p, _i64, _p]),
     "k2q_sigmoid_gate_bwd": (C.c_int, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p]),
     "k2q_gate_residual": (C.c_int, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _i64, _p]),
+    "k2q_residual_norm_quant": (C.c_int, [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _f, _p, _i64, _p, _p, _p]),
+    "k2q_residual_norm_fwd": (C.c_int, [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _p,
+                                        _p]),
+    "k2q_residual_norm_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "k2q_residual_norm_bwd": (C.c_int, [_p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _i64,
+                                        _p, _i64, _p, _p, _p, _p, _p, _i64, _p]),
     "k2q_requant_i4_to_i8": (C.c_int, [_p, _p, _i64, _i64, _p, _i64, _p, _p]),
     "k2q_gemm_dx_w8": (C.c_int, [_p, _p, _i64, _i64, _i64, C.POINTER(Epilogue), _p, _i64, _p, _p]),
     "k2q_transpose_i8": (C.c_int, [_p, _i64, _i64, _p, _p]),

@@ -11,6 +11,8 @@ modulation vector that itself needs a gradient):
     swiglu(g, u)                                silu(g) * u                            mmdit.py:178
     sigmoid_gate(a, g)                          a * sigmoid(g)                         mmdit.py:210
     gate_residual(x, gate, y)                   x + gate * y                           mmdit.py:318-321
+    residual_norm(x, y, ...)                    the last and the first of these as one step, with the
+                                                gradients of every vector                mmdit.py:310-321
 """
 from __future__ import annotations
 
@@ -18,9 +20,10 @@ import ctypes as C
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _ptr, _stream
+from .ops import _aligned_rows, _check_residual, _mod_vec, _ptr, _row_stride, _stream
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -229,4 +232,107 @@ def gate_residual(x: torch.Tensor, gate: torch.Tensor, y: torch.Tensor) -> torch
     return x + gate * y
 
 
-__all__ = ["norm_modulate", "qk_norm_rope_train", "qk_norm_rope_trainable", "swiglu", "sigmoid_gate", "gate_residual"]
+# ---------------------------------------------------------------------------------------------
+# gated residual + RMSNorm + modulation, one kernel each way
+# ---------------------------------------------------------------------------------------------
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, norm_scale, gate, mod_scale, mod_shift, eps):
+        k = x.shape[-1]
+        m = x.numel() // k
+        rows = x.shape[-2] if x.dim() >= 3 else m
+        nb = m // rows
+        x2, y2 = _aligned_rows(x), _aligned_rows(y)
+        w = norm_scale if norm_scale.data_ptr() % 16 == 0 else norm_scale.clone()
+        g, sc, sh = (_mod_vec("residual_norm", n, t, nb, k) for n, t in (("gate", gate), ("mod_scale", mod_scale),
+                                                                         ("mod_shift", mod_shift)))
+        stream = torch.empty(m, k, dtype=torch.bfloat16, device=x.device)
+        h = torch.empty(m, k, dtype=torch.bfloat16, device=x.device)
+        rstd = torch.empty(m, dtype=torch.float32, device=x.device)
+        _call("k2q_residual_norm_fwd", x.device, _ptr(x2), _row_stride(x2), _ptr(y2), _row_stride(y2), _ptr(g), _ptr(w),
+              _ptr(sc), _ptr(sh), rows, m, k, float(eps), _ptr(stream), k, _ptr(h), k, _ptr(rstd))
+        stream, h = stream.view(x.shape), h.view(x.shape)
+        ctx.save_for_backward(stream, rstd, w, g, sc, y2 if gate is not None and gate.requires_grad else None)
+        ctx.rows = rows
+        ctx.shapes = tuple(None if t is None else t.shape for t in (x, norm_scale, gate, mod_scale, mod_shift))
+        ctx.set_materialize_grads(False)
+        return stream, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, ds, dh):
+        stream, rstd, w, g, sc, y2 = ctx.saved_tensors
+        if ds is None and dh is None:
+            return (None,) * 7
+        need_x, need_y, need_w, need_g, need_sc, need_sh, _ = ctx.needs_input_grad
+        xs, ws_, gs, scs, shs = ctx.shapes
+        k = xs[-1]
+        m = stream.numel() // k
+        dev = stream.device
+        nb = m // ctx.rows
+
+        def grad_rows(t):
+            return None if t is None else _aligned_rows(t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16))
+
+        ds2, dh2, s2 = grad_rows(ds), grad_rows(dh), stream.view(m, k)
+        bf = dict(dtype=torch.bfloat16, device=dev)
+        same = g is None                               # without a gate dy equals dx: one tensor serves both
+        dx = torch.empty(m, k, **bf) if need_x or (same and need_y) else None
+        dy = torch.empty(m, k, **bf) if need_y and not same else None
+        dg = torch.empty(nb, k, **bf) if need_g else None
+        dsc = torch.empty(nb, k, **bf) if need_sc else None
+        dsh = torch.empty(nb, k, **bf) if need_sh else None
+        dw = torch.empty(k, dtype=torch.float32, device=dev) if need_w else None
+        ws = None
+        ws_bytes = 0
+        if need_g or need_sc or need_sh or need_w:
+            ws_bytes = int(_lib.load().k2q_residual_norm_bwd_workspace_bytes(ctx.rows, m, k))
+            ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=dev)
+
+        def ld(t):
+            return 0 if t is None else _row_stride(t)
+
+        _call("k2q_residual_norm_bwd", dev, _ptr(ds2), ld(ds2), _ptr(dh2), ld(dh2), _ptr(s2), k, _ptr(rstd), _ptr(y2), ld(y2),
+              _ptr(g), _ptr(w), _ptr(sc), ctx.rows, m, k, _ptr(dx), k, _ptr(dy), k, _ptr(dg), _ptr(dsc), _ptr(dsh), _ptr(dw),
+              _ptr(ws), ws_bytes)
+
+        def like(t, shape):
+            return None if t is None else t.view(shape)
+
+        dxv = like(dx, xs)
+        return (dxv if need_x else None, (dxv if same else like(dy, xs)) if need_y else None, like(dw, ws_), like(dg, gs),
+                like(dsc, scs), like(dsh, shs), None)
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor, norm_scale: torch.Tensor, gate: torch.Tensor | None = None,
+                  mod_scale: torch.Tensor | None = None, mod_shift: torch.Tensor | None = None, eps: float = 1e-5):
+    """``(stream, h)`` with ``stream = x + gate * y`` and ``h = (1 + mod_scale) * RMSNorm(stream) + mod_shift``: what
+    a block does between two of its halves (mmdit.py:310-321; without vectors mmdit.py:237-246), forward and
+    backward one kernel each.  x, y [..., L, K]; norm_scale fp32 [K] (weight 1 + norm_scale); gate / mod_scale /
+    mod_shift [B, 1, K] or [B, K], each or None.  Any of the inputs may need a gradient.  fp32 inside, the
+    stream rounded once where it is kept.  Where the kernel does not apply (CPU, other types, K not a
+    multiple of 8 or above 16384) the same expression runs op by op."""
+    k = x.shape[-1]
+    vectors = (gate, mod_scale, mod_shift)
+    if _kernel_ok(x, y, *vectors) and norm_scale.is_cuda and norm_scale.dtype == torch.float32 and k % 8 == 0 and 0 < k <= 16384 \
+            and x.numel() > 0:
+        _check_residual("residual_norm", x, y, norm_scale, k)
+        if len({t.device for t in (x, y, norm_scale, *vectors) if t is not None}) != 1:
+            raise RuntimeError("residual_norm: tensors on different devices")
+        return _ResidualNorm.apply(x, y, norm_scale, gate, mod_scale, mod_shift, eps)
+    lead = x.shape[:-2] if x.dim() >= 3 else ()
+
+    def vec(t):
+        return t.float().reshape(*lead, 1, k)
+
+    s = (x.float() + (y.float() if gate is None else vec(gate) * y.float())).to(x.dtype)
+    v = s.float()
+    h = v * torch.rsqrt(v.square().mean(-1, keepdim=True) + eps) * (1.0 + norm_scale.float())
+    if mod_scale is not None:
+        h = h * (1.0 + vec(mod_scale))
+    if mod_shift is not None:
+        h = h + vec(mod_shift)
+    return s, h.to(x.dtype)
+
+
+__all__ = ["residual_norm", "norm_modulate", "qk_norm_rope_train", "qk_norm_rope_trainable", "swiglu", "sigmoid_gate", "gate_residual"]

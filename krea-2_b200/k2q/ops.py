@@ -247,6 +247,105 @@ def norm_mod_quant(x: torch.Tensor, norm_scale: torch.Tensor, mod_scale: torch.T
     return xq, sx
 
 
+def _mod_vec(name: str, what: str, t: torch.Tensor | None, nb: int, k: int) -> torch.Tensor | None:
+    """A per-sample vector [B, 1, K] / [B, K] as contiguous [B, K] with a 16-byte aligned base."""
+    if t is None:
+        return None
+    if t.dtype != torch.bfloat16 or t.numel() != nb * k or t.shape[-1] != k:
+        raise ValueError(f"{name}: {what} must be bf16 with {nb} x {k} elements")
+    t = t.reshape(nb, k).contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """[..., K] -> [rows, K] with unit inner stride, a row stride of whole 16-byte pieces and an aligned base."""
+    t2 = t.reshape(-1, t.shape[-1])
+    if (t2.stride(1) != 1 or t2.data_ptr() % 16
+            or (t2.shape[0] > 1 and (t2.stride(0) % 8 or t2.stride(0) < t2.shape[1]))):
+        t2 = t2.clone(memory_format=torch.contiguous_format)
+    return t2
+
+
+def _row_stride(t2: torch.Tensor) -> int:
+    """Leading dimension of a [rows, K] matrix (a single row may carry any stride)."""
+    return t2.stride(0) if t2.shape[0] > 1 else t2.shape[1]
+
+
+def _span(t: torch.Tensor):
+    """First and last byte of a row matrix."""
+    return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * _row_stride(t) + t.shape[1]) * t.element_size()
+
+
+def _check_residual(name, x, y, norm_scale, k):
+    if x.dtype != torch.bfloat16 or y.dtype != torch.bfloat16 or x.dim() < 2 or x.shape != y.shape:
+        raise ValueError(f"{name}: x and y must be bf16 tensors [..., L, K] of one shape")
+    if norm_scale.dtype != torch.float32 or norm_scale.numel() != k or not norm_scale.is_contiguous():
+        raise ValueError(f"{name}: norm_scale must be a contiguous fp32 vector of length K")
+
+
+def residual_norm_quant(x: torch.Tensor, y: torch.Tensor, norm_scale: torch.Tensor, gate: torch.Tensor | None = None,
+                        mod_scale: torch.Tensor | None = None, mod_shift: torch.Tensor | None = None, eps: float = 1e-5,
+                        out: torch.Tensor | None = None):
+    """Residual update, RMS norm, modulation, rotation and 8-bit quantisation of a block in one pass
+    (mmdit.py:310-321; without vectors the plain addition and norm of mmdit.py:237-246):
+
+        stream = bf16(x + gate * y)
+        codes, scales of  (1 + mod_scale) * RMSNorm(stream) + mod_shift
+
+    for x, y [..., L, K] bf16 (K a multiple of 128 up to 16384), norm_scale [K] fp32 (weight 1 + norm_scale),
+    gate / mod_scale / mod_shift [B, 1, K] or [B, K] bf16 with B = the product of the dimensions in front of L
+    (each, or None).  Returns (stream like x, int8 codes [M, K], fp32 scales [M]).  ``out`` receives the stream;
+    it may be x or y itself (in place).  Everything between loads and stores is fp32: the codes differ
+    in rounding from ``norm_mod_quant(gate_residual(...))``, which rounds to bf16 after every step."""
+    name = "residual_norm_quant"
+    dev = _need_cuda(x, y, norm_scale, gate, mod_scale, mod_shift, out)
+    k = x.shape[-1]
+    _check_residual(name, x, y, norm_scale, k)
+    if k % HAD_BLOCK or k > 16384 or k == 0:
+        raise ValueError(f"{name}: K={k} must be a multiple of {HAD_BLOCK} up to 16384")
+    m = x.numel() // k
+    xq = torch.empty(m, k, dtype=torch.int8, device=dev)
+    sx = torch.empty(m, dtype=torch.float32, device=dev)
+    if out is not None and (out.dtype != torch.bfloat16 or out.shape != x.shape):
+        raise ValueError(f"{name}: out must be a bf16 tensor of x's shape")
+    if m == 0:
+        return (torch.empty_like(x) if out is None else out), xq, sx
+    rows = x.shape[-2] if x.dim() >= 3 else m
+    x2, y2 = _aligned_rows(x), _aligned_rows(y)
+    if out is None:
+        o2 = torch.empty(m, k, dtype=torch.bfloat16, device=dev)
+        out = o2.view(x.shape)
+    else:
+        o2 = _out_rows(name, out, k)
+        for what, src in (("x", x2), ("y", y2)):
+            (a0, a1), (b0, b1) = _span(o2), _span(src)
+            if a0 < b1 and b0 < a1 and not (a0 == b0 and _row_stride(o2) == _row_stride(src)):
+                raise ValueError(f"{name}: out overlaps {what} without being {what}")
+        note_raw_write()
+    if norm_scale.data_ptr() % 16:
+        norm_scale = norm_scale.clone()
+    g, sc, sh = (_mod_vec(name, w, t, m // rows, k) for w, t in (("gate", gate), ("mod_scale", mod_scale),
+                                                                 ("mod_shift", mod_shift)))
+    with torch.cuda.device(dev):
+        rc = _lib.load().k2q_residual_norm_quant(
+            _ptr(x2), _row_stride(x2), _ptr(y2), _row_stride(y2), _ptr(g), _ptr(norm_scale), _ptr(sc), _ptr(sh), rows, m, k,
+            float(eps), _ptr(o2), _row_stride(o2), _ptr(xq), _ptr(sx), _stream(dev))
+    _lib.check(rc, "k2q_residual_norm_quant")
+    return out, xq, sx
+
+
+def _out_rows(name: str, out: torch.Tensor, k: int) -> torch.Tensor:
+    """``out`` as the [rows, K] matrix a kernel writes; no copy may be made of it."""
+    try:
+        o2 = out.view(-1, k)
+    except RuntimeError:
+        o2 = None
+    if (o2 is None or o2.stride(1) != 1 or o2.data_ptr() % 16
+            or (o2.shape[0] > 1 and (o2.stride(0) % 8 or o2.stride(0) < k))):
+        raise ValueError(f"{name}: out needs rows of unit stride, 16-byte aligned, one stride apart")
+    return o2
+
+
 def qknorm_rope_(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor,
                  cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, eps: float = 1e-5) -> None:
     """In place: QK-RMSNorm (weights 1 + wq / 1 + wk, fp32 [128]) and the rotary embedding of
