@@ -220,6 +220,13 @@ int k2q_gemm_w4a8(const int8_t* xq, const uint8_t* wq4, const void* sw4_bf16, in
                   int64_t N, int64_t K, const k2q_epilogue* ep, void* y_bf16, int64_t ldy,
                   void* status, void* stream);
 
+/* K4 for a few token rows (M <= 32: the timestep MLP and projection, mmdit.py:360-375, short prompts): the
+ * same operands, epilogue and BITS as k2q_gemm_w4a8 -- exact integer group sums, scales folded in ascending
+ * order of the groups -- in a kernel bound by reading the codes once.  xq and wq4 16-byte aligned; sw4, sx and bias
+ * need no alignment beyond their type's.  No waits on other threads' progress, hence no status block.       */
+int k2q_gemv_w4a8(const int8_t* xq, const uint8_t* wq4, const void* sw4_bf16, int64_t M, int64_t N, int64_t K,
+                  const k2q_epilogue* ep, void* y_bf16, int64_t ldy, void* stream);
+
 /* Backward of K3 through the SAME stored codes (autograd of quantize.py:51, dX = dY . w):
  *   dx[m,k] = acc[m,k]*sx[m] + lora_scale * sum_j u[m,j]*Bm[k,j],   acc = sum_n gq[m,n]*wq[n,k]
  * gq [M, N] int8 = per-token quantised dY*sw (k2q_quant_rows_i8, scale in ep->sx), wq [N, K] int8 exactly
@@ -325,6 +332,37 @@ int k2q_sumsq_f32(const float* g, int64_t n, float* out, int accumulate, void* w
 int k2q_adamw_clip_f32(float* p, float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2,
                        float eps, float weight_decay, int64_t step, float max_norm, const float* normsq_dev,
                        int zero_grad, void* stream);
+
+/* ---- orthogonalised optimizer step of the adapters (no counterpart in the reference, which steps them with
+ * AdamW: train_t2i_lora_cached.py:143, 327-332; the update of the Muon optimiser) ------------------------
+ * `count` matrices rows[i] x cols[i] lie end to end, row-major, in flat fp32 buffers; the short side of
+ * each is 1 to 64, the other any length.  Per matrix, with beta the momentum:
+ *   m = beta m + (1 - beta) g;   u = nesterov ? beta m + (1 - beta) g : m;   X = u / (||u||_F + eps)
+ *   `steps` times (0 to 10):  X = (a I + b X X^T + c (X X^T)^2) X on the short side, a, b, c = 3.4445, -4.7750, 2.0315
+ *   p = p (1 - lr weight_decay) - lr s X,   s = 0.2 sqrt(max(rows, cols)) (scale_mode 0) or
+ *                                               sqrt(max(1, rows / cols)) (scale_mode 1)
+ * g is first scaled by min(1, max_norm / (sqrt(*normsq_dev) + 1e-6)) (max_norm <= 0 or normsq_dev NULL: not),
+ * and zeroed at the end when zero_grad != 0.  A matrix whose u is zero moves by its weight decay alone; one
+ * with a NaN, or whose sum of squares leaves the fp32 range, becomes NaN and leaves the others alone.
+ * k2q_orthogonalize gives X of a given u (out may be u).  All sums are formed in a fixed order.
+ *   k2q_matrices_plan    host only: sizes of the table and the workspace for these shapes
+ *   k2q_matrices_table   host only: fills table_host (plan.table_bytes); the caller copies it to 16-byte aligned
+ *                        device memory once, it depends on the shapes alone and is only read
+ * The workspace (16-byte aligned, plan.workspace_bytes) belongs to one call at a time.                    */
+typedef struct k2q_matrices {
+  int64_t count, total;                  /* matrices; elements of a flat buffer            */
+  int64_t table_bytes, workspace_bytes;
+  int64_t piece, tiles;                  /* columns per piece of a long side; pieces       */
+  int32_t max_short, pad_;
+} k2q_matrices;
+
+int k2q_matrices_plan(const int64_t* rows, const int64_t* cols, int64_t count, k2q_matrices* plan);
+int k2q_matrices_table(const int64_t* rows, const int64_t* cols, int64_t count, void* table_host, int64_t table_bytes);
+int k2q_orthogonal_step(float* p, float* g, float* m, const k2q_matrices* plan, const void* table, float lr, float beta,
+                        int nesterov, float weight_decay, int scale_mode, int steps, float eps, float max_norm,
+                        const float* normsq_dev, int zero_grad, void* ws, int64_t ws_bytes, void* stream);
+int k2q_orthogonalize(const float* u, float* out, const k2q_matrices* plan, const void* table, int steps, float eps,
+                      void* ws, int64_t ws_bytes, void* stream);
 
 /* ---- self-test of the bounded waits (no counterpart in the reference) ------------------------
  * Launches one warp that waits, with a limit of a few microseconds, on a barrier nobody signals.

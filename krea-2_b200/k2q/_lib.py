@@ -43,6 +43,20 @@ class Linear(C.Structure):
     ]
 
 
+class Matrices(C.Structure):
+    """``struct k2q_matrices`` of include/k2q.h."""
+    _fields_ = [
+        ("count", C.c_int64),
+        ("total", C.c_int64),
+        ("table_bytes", C.c_int64),
+        ("workspace_bytes", C.c_int64),
+        ("piece", C.c_int64),
+        ("tiles", C.c_int64),
+        ("max_short", C.c_int32),
+        ("pad_", C.c_int32),
+    ]
+
+
 _i64, _i32, _p, _f = C.c_int64, C.c_int32, C.c_void_p, C.c_float
 
 # name -> (restype, argtypes); every symbol include/k2q.h declares
@@ -61,6 +75,7 @@ SIGNATURES = {
     "k2q_fwht_rows": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _p, C.c_int, _i64, _p]),
     "k2q_gemm_w8a8": (C.c_int, [_p, _p, _p, _i64, _i64, _i64, C.POINTER(Epilogue), _p, _i64, _p, _p]),
     "k2q_gemm_w4a8": (C.c_int, [_p, _p, _p, _i64, _i64, _i64, C.POINTER(Epilogue), _p, _i64, _p, _p]),
+    "k2q_gemv_w4a8": (C.c_int, [_p, _p, _p, _i64, _i64, _i64, C.POINTER(Epilogue), _p, _i64, _p]),
     "k2q_qknorm_rope": (C.c_int, [_p, _i64, C.c_int, _p, _p, _i64, C.c_int, _p, _i64, _p, _p, C.c_float, _p]),
     "k2q_norm_mod_fwd": (C.c_int, [_p, _i64, _i64, _i64, _p, _p, _p, _i64, C.c_float, _p, _i64, _p, _p]),
     "k2q_norm_mod_bwd": (C.c_int, [_p, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _p]),
@@ -92,6 +107,11 @@ SIGNATURES = {
     "k2q_sumsq_workspace_bytes": (_i64, []),
     "k2q_sumsq_f32": (C.c_int, [_p, _i64, _p, C.c_int, _p, _i64, _p]),
     "k2q_adamw_clip_f32": (C.c_int, [_p, _p, _p, _p, _i64, _f, _f, _f, _f, _f, _i64, _f, _p, C.c_int, _p]),
+    "k2q_matrices_plan": (C.c_int, [C.POINTER(_i64), C.POINTER(_i64), _i64, C.POINTER(Matrices)]),
+    "k2q_matrices_table": (C.c_int, [C.POINTER(_i64), C.POINTER(_i64), _i64, _p, _i64]),
+    "k2q_orthogonal_step": (C.c_int, [_p, _p, _p, C.POINTER(Matrices), _p, _f, _f, C.c_int, _f, C.c_int, C.c_int, _f, _f, _p,
+                                      C.c_int, _p, _i64, _p]),
+    "k2q_orthogonalize": (C.c_int, [_p, _p, C.POINTER(Matrices), _p, C.c_int, _f, _p, _i64, _p]),
     "k2q_selftest_wait_expiry": (C.c_int, [_p, C.c_int, _p]),
     "k2q_fwht_quant_act_i8_stream_ok": (C.c_int, [C.c_int, _i64, _i64, _i64]),
     "k2q_fwht_quant_act_i8_stream": (C.c_int, [_p, _i64, _i64, _p, _p, _p, _p]),

@@ -478,21 +478,27 @@ def gemm_w8a8(xq, sx, wq, sw, bias=None, u=None, bm=None, lora_scale: float = 0.
     return y
 
 
+def _check_w4a8(name, xq, sx, wq4, sw4, bias, u, bm):
+    """Operands of a W4A8 product; returns (M, N, K)."""
+    m, k = xq.shape
+    n = wq4.shape[0]
+    if wq4.shape[1] * 2 != k or xq.dtype != torch.int8 or wq4.dtype != torch.uint8:
+        raise ValueError(f"{name}: xq [M,K] int8 and wq4 [N,K/2] uint8 expected")
+    if sw4.dtype != torch.bfloat16 or tuple(sw4.shape) != (n, k // GROUP) or not sw4.is_contiguous():
+        raise ValueError(f"{name}: sw4 must be contiguous bf16 [N, K/128]")
+    if not (xq.is_contiguous() and wq4.is_contiguous()):
+        raise ValueError(f"{name}: codes must be contiguous")
+    _check_vec("sx", sx, m)
+    _check_vec("bias", bias, n)
+    _check_lora(name, u, bm, m, n)
+    return m, n, k
+
+
 def gemm_w4a8(xq, sx, wq4, sw4, bias=None, u=None, bm=None, lora_scale: float = 0.0, act=None,
               out: torch.Tensor | None = None) -> torch.Tensor:
     """W4A8 variant: wq4 [N,K/2] packed uint8, sw4 [N,K/128] bf16."""
     dev = _need_cuda(xq, sx, wq4, sw4, bias, u, bm)
-    m, k = xq.shape
-    n = wq4.shape[0]
-    if wq4.shape[1] * 2 != k or xq.dtype != torch.int8 or wq4.dtype != torch.uint8:
-        raise ValueError("gemm_w4a8: xq [M,K] int8 and wq4 [N,K/2] uint8 expected")
-    if sw4.dtype != torch.bfloat16 or tuple(sw4.shape) != (n, k // GROUP) or not sw4.is_contiguous():
-        raise ValueError("gemm_w4a8: sw4 must be contiguous bf16 [N, K/128]")
-    if not (xq.is_contiguous() and wq4.is_contiguous()):
-        raise ValueError("gemm_w4a8: codes must be contiguous")
-    _check_vec("sx", sx, m)
-    _check_vec("bias", bias, n)
-    _check_lora("gemm_w4a8", u, bm, m, n)
+    m, n, k = _check_w4a8("gemm_w4a8", xq, sx, wq4, sw4, bias, u, bm)
     if out is not None:
         _check_out("gemm_w4a8", out, m, n, dev)
     y = out if out is not None else torch.empty(m, n, dtype=torch.bfloat16, device=dev)
@@ -501,6 +507,31 @@ def gemm_w4a8(xq, sx, wq4, sw4, bias=None, u=None, bm=None, lora_scale: float = 
         rc = _lib.load().k2q_gemm_w4a8(_ptr(xq), _ptr(wq4), _ptr(sw4), m, n, k, C.byref(ep), _ptr(y), y.stride(0),
                                        _ptr(status_block(dev)), _stream(dev))
     _lib.check(rc, "k2q_gemm_w4a8")
+    return y
+
+
+GEMV_ROWS = 32        # token rows that gemv_w4a8 takes
+
+
+def gemv_w4a8(xq, sx, wq4, sw4, bias=None, u=None, bm=None, lora_scale: float = 0.0, act=None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`gemm_w4a8` for up to ``GEMV_ROWS`` token rows (one timestep vector per image, a short prompt): the
+    same operands and the same bits, from a kernel that is bound by reading the 4-bit codes once."""
+    name = "gemv_w4a8"
+    dev = _need_cuda(xq, sx, wq4, sw4, bias, u, bm)
+    m, n, k = _check_w4a8(name, xq, sx, wq4, sw4, bias, u, bm)
+    if m > GEMV_ROWS:
+        raise ValueError(f"{name}: {m} token rows; it takes up to {GEMV_ROWS} (gemm_w4a8 takes any number)")
+    if out is not None:
+        _check_out(name, out, m, n, dev)
+    y = out if out is not None else torch.empty(m, n, dtype=torch.bfloat16, device=dev)
+    if m == 0:
+        return y
+    ep = _epilogue(sx, bias, u, bm, lora_scale, act)
+    with torch.cuda.device(dev):
+        rc = _lib.load().k2q_gemv_w4a8(_ptr(xq), _ptr(wq4), _ptr(sw4), m, n, k, C.byref(ep), _ptr(y),
+                                       y.stride(0) if m > 1 else n, _stream(dev))
+    _lib.check(rc, "k2q_gemv_w4a8")
     return y
 
 
@@ -633,6 +664,98 @@ def lora_tn(p: torch.Tensor, q: torch.Tensor, scale: float = 1.0) -> torch.Tenso
         rc = lib.k2q_lora_tn(_ptr(p2), p2.stride(0), _ptr(q2), q2.stride(0), t, r, c, float(scale), _ptr(out), c,
                              _ptr(ws), ws_bytes, _stream(dev))
     _lib.check(rc, "k2q_lora_tn")
+    return out
+
+
+# --------------------------------------------------------------------------------------------
+# orthogonalised update of flat adapter buffers
+# --------------------------------------------------------------------------------------------
+class MatrixLayout:
+    """Matrices lying end to end, row-major, in flat fp32 buffers (adapters' A [r, K] and B [N, r] in the order
+    of their gradient buckets): what the kernels of :func:`orthogonal_step_` need to know about them, held
+    on the device.  The short side of each is 1 to 64.  It depends on the shapes alone and is only read, so
+    one layout serves any number of buffers, streams and captured graphs; make it outside stream capture."""
+
+    def __init__(self, shapes, device):
+        shapes = [tuple(int(v) for v in s) for s in shapes]
+        if not shapes or any(len(s) != 2 for s in shapes):
+            raise ValueError("MatrixLayout: a list of (rows, cols) expected")
+        n = len(shapes)
+        lib = _lib.load()
+        rows, cols = (C.c_int64 * n)(*(s[0] for s in shapes)), (C.c_int64 * n)(*(s[1] for s in shapes))
+        self.plan = _lib.Matrices()
+        _lib.check(lib.k2q_matrices_plan(rows, cols, n, C.byref(self.plan)), "k2q_matrices_plan")
+        table = torch.empty(self.plan.table_bytes // 8, dtype=torch.int64)
+        _lib.check(lib.k2q_matrices_table(rows, cols, n, _ptr(table), self.plan.table_bytes), "k2q_matrices_table")
+        self.shapes = shapes
+        self.numel = int(self.plan.total)
+        self.table = table.to(device)
+
+
+def _check_flat(name: str, layout: MatrixLayout, **tensors) -> torch.device:
+    dev = _need_cuda(*tensors.values(), layout.table)
+    for what, t in tensors.items():
+        if t.dtype != torch.float32 or t.numel() != layout.numel or not t.is_contiguous():
+            raise ValueError(f"{name}: {what} must be a contiguous fp32 buffer of {layout.numel} elements")
+    return dev
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() < b.data_ptr() + b.numel() * 4 and b.data_ptr() < a.data_ptr() + a.numel() * 4
+
+
+_STEP_SCALES = {"rms": 0, "spectral": 1}
+
+
+def orthogonal_step_(param: torch.Tensor, grad: torch.Tensor, moment: torch.Tensor, layout: MatrixLayout, lr: float,
+                     momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, scale: str = "rms",
+                     steps: int = 5, eps: float = 1e-7, max_norm: float = 0.0, normsq: torch.Tensor | None = None,
+                     zero_grad: bool = False) -> None:
+    """In place, for every matrix of ``layout`` in the flat buffers ``param``, ``grad``, ``moment``: the momentum
+    update, the Newton-Schulz orthogonalisation of the (Nesterov) momentum on the matrix's short side, and
+
+        param = param * (1 - lr * weight_decay) - lr * s * X
+
+    with s = 0.2 sqrt(max(rows, cols)) (``scale="rms"``: an update of AdamW's usual size) or
+    sqrt(max(1, rows / cols)) (``"spectral"``).  ``normsq`` (device scalar, the sum of squares of all gradients)
+    with ``max_norm`` > 0 clips as ``clip_grad_norm_`` does; ``zero_grad`` zeroes the gradients at the end.
+    A matrix with a zero momentum moves by its weight decay alone."""
+    name = "orthogonal_step_"
+    dev = _check_flat(name, layout, param=param, grad=grad, moment=moment)
+    if any(_overlap(a, b) for a, b in ((param, grad), (param, moment), (grad, moment))):
+        raise ValueError(f"{name}: param, grad and moment must be three buffers")
+    if scale not in _STEP_SCALES:
+        raise ValueError(f"{name}: scale must be one of {sorted(_STEP_SCALES)}, got {scale!r}")
+    if normsq is not None and (normsq.dtype != torch.float32 or normsq.numel() != 1 or normsq.device != dev):
+        raise ValueError(f"{name}: normsq must be one fp32 value on the buffers' device")
+    pl = layout.plan
+    ws = torch.empty(pl.workspace_bytes // 4, dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        rc = _lib.load().k2q_orthogonal_step(
+            _ptr(param), _ptr(grad), _ptr(moment), C.byref(pl), _ptr(layout.table), float(lr), float(momentum), int(bool(nesterov)),
+            float(weight_decay), _STEP_SCALES[scale], int(steps), float(eps), float(max_norm), _ptr(normsq),
+            int(bool(zero_grad)), _ptr(ws), ws.numel() * 4, _stream(dev))
+    _lib.check(rc, "k2q_orthogonal_step")
+    note_raw_write()
+
+
+def orthogonalize(u: torch.Tensor, layout: MatrixLayout, steps: int = 5, eps: float = 1e-7,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """The Newton-Schulz orthogonalisation of every matrix of ``layout`` in the flat fp32 buffer ``u`` (``out`` may be
+    ``u``): singular values are moved towards one, singular vectors kept."""
+    name = "orthogonalize"
+    if out is None:
+        out = torch.empty_like(u)
+    dev = _check_flat(name, layout, u=u, out=out)
+    if _overlap(u, out) and u.data_ptr() != out.data_ptr():
+        raise ValueError(f"{name}: out overlaps u without being u")
+    pl = layout.plan
+    ws = torch.empty(pl.workspace_bytes // 4, dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        rc = _lib.load().k2q_orthogonalize(_ptr(u), _ptr(out), C.byref(pl), _ptr(layout.table), int(steps), float(eps), _ptr(ws),
+                                           ws.numel() * 4, _stream(dev))
+    _lib.check(rc, "k2q_orthogonalize")
+    note_raw_write()
     return out
 
 
