@@ -6,13 +6,25 @@
 // The group sums are exact integers and the scales enter in ascending order of the groups, one fused
 // multiply-add each: the operations of the large W4A8 product on every element, so both give the same bits.
 // Bound by reading the codes once: N*K/2 bytes.
+//
+// A warp owns 8 or 16 channels over the whole contraction and folds every group in registers; nothing is
+// exchanged between warps.  A group of eight channels is four m16n8k32 int8 MMAs per 16 tokens, the tokens as
+// rows.  The order of k inside a group is free as long as both operands agree, so a lane simply takes 16
+// consecutive bytes of a channel (32 codes): the low nibbles of a word, shifted up, and its high nibbles are two
+// operand registers holding 16 times the codes, and the tokens' bytes are dealt out to match (even and odd
+// bytes of eight).
+//   - The codes travel by 16-byte asynchronous copies into a ring of shared memory; a lane reads back
+//     only what it copied itself, so the ring needs no barrier and stays full whatever the arithmetic does.
+//   - The tokens and the scales are staged in shared memory beforehand.  Plain loads of them inside the loop return
+//     in order behind the codes' misses in the L1 pipe and cost each group a trip to DRAM (measured: 520 ns a
+//     group); copies of them in the ring, several lanes from one address, were slower still.
 #include "k2q_common.cuh"
 
 namespace k2q {
 namespace {
 
 constexpr int kMaxRows = 32;
-constexpr int kWarps = 4;
+constexpr int kMaxK = 131072;         // the scales of 16 channels stay in shared memory: K / 4 bytes
 
 struct GemvParams {
   int M, N, K;
@@ -20,6 +32,8 @@ struct GemvParams {
   const float* sx; const float* bias; const float* u; const float* Bm;
   int64_t ldu, ldb; int rank; float lora_scale; int act;
   __nv_bfloat16* y; int64_t ldy;
+  int warps;                          // warps per CTA that multiply
+  int chunk;                          // groups of the tokens staged at a time
 };
 
 // the activation of the large product: hardware tanh, |error| < 6e-4, below the bf16 step of the output
@@ -43,26 +57,217 @@ __device__ __forceinline__ void finish(const GemvParams& p, int m, int n, float 
   p.y[m * p.ldy + n] = __float2bfloat16_rn(v);
 }
 
-// One warp per output channel; a lane holds four codes of the group, the group sums are added over the
-// warp, and lane m keeps the running value of token m.
-__global__ void __launch_bounds__(kWarps * 32) gemv_kernel(const GemvParams p) {
-  const int lane = threadIdx.x & 31;
-  const int n = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (n >= p.N) return;
+__device__ __forceinline__ void mma_s8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pick(uint32_t a, uint32_t b, uint32_t sel) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+  return r;
+}
+
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+constexpr int kMaxWarps = 16;
+constexpr int kSmemMax = 232448;
+
+// Groups [g0, g0 + chunk) of every token into shared memory, the even and the odd bytes of every eight apart.  A
+// token's row there is chunk * 128 + 16 bytes long: the eight lanes of a 16-byte read phase (two tokens, four
+// quarters of a group) meet 32 different banks.
+__device__ __forceinline__ void request_tokens(const GemvParams& p, uint32_t xs, int g0) {
+  const int n = min(p.chunk, (p.K >> 7) - g0) * 8, row = p.chunk * 128 + 16;      // n 16-byte pieces per token
+  const int8_t* src = p.xq + g0 * 128LL;
+  for (int e = threadIdx.x, m = e / n, c = e - m * n; m < p.M;) {
+    cp_async16(xs + m * row + c * 16, src + static_cast<int64_t>(m) * p.K + c * 16, 16);
+    for (c += blockDim.x; c >= n; c -= n) ++m;
+  }
+}
+// after this thread's copies have arrived
+__device__ __forceinline__ void deal_tokens(const GemvParams& p, uint8_t* xs, int g0) {
+  const int n = min(p.chunk, (p.K >> 7) - g0) * 8, row = p.chunk * 128 + 16;
+  for (int e = threadIdx.x, m = e / n, c = e - m * n; m < p.M;) {
+    uint4* at = reinterpret_cast<uint4*>(xs + m * row + c * 16);
+    const uint4 v = *at;
+    *at = make_uint4(pick(v.x, v.y, 0x6420u), pick(v.x, v.y, 0x7531u), pick(v.z, v.w, 0x6420u), pick(v.z, v.w, 0x7531u));
+    for (c += blockDim.x; c >= n; c -= n) ++m;
+  }
+}
+
+// MH halves of eight tokens, CT tiles of eight channels per warp, RING entries of GP groups.
+template <int MH, int CT, int GP, int RING>
+__global__ void __launch_bounds__(kMaxWarps * 32, 1) gemv_kernel(const GemvParams p) {
+  constexpr int MT = (MH + 1) / 2;                             // tiles of 16 tokens
+  constexpr uint32_t kEntry = CT * GP * 512;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3, warps = p.warps;
   const int groups = p.K >> 7;
-  float run = 0.f;
-  for (int g = 0; g < groups; ++g) {
-    const uint32_t c = __ldg(reinterpret_cast<const uint16_t*>(p.wq + static_cast<int64_t>(n) * (p.K >> 1) + g * 64) + lane);
-    // codes k0, k1, k2, k3 as the high nibbles of four bytes: 16 times their value
-    const int w = static_cast<int>(((c << 4) & 0xF0u) | ((c & 0xF0u) << 8) | ((c & 0x0F00u) << 12) | ((c & 0xF000u) << 16));
-    const float s = __bfloat162float(p.sw[static_cast<int64_t>(n) * groups + g]) * 0.0625f;
-    for (int m = 0; m < p.M; ++m) {
-      const int x = __ldg(reinterpret_cast<const int*>(p.xq + static_cast<int64_t>(m) * p.K + g * 128) + lane);
-      const int acc = __reduce_add_sync(0xffffffffu, __dp4a(x, w, 0));
-      if (lane == m) run = fmaf(static_cast<float>(acc), s, run);
+  const int n0 = (blockIdx.x * warps + warp) * (8 * CT);
+  const bool live = warp < warps && n0 < p.N;                  // the other warps only help to stage the tokens
+  // shared memory: rings | scales [channel][group] | tokens
+  const uint32_t ring = smem_u32(smem) + warp * (RING * kEntry) + lane * 16;
+  uint8_t* scales = smem + warps * RING * kEntry;
+  uint8_t* xs = scales + warps * groups * (16 * CT);
+  pdl_wait();
+  request_tokens(p, smem_u32(xs), 0);
+  {
+    const int first = blockIdx.x * warps * (8 * CT), n = min(warps * 8 * CT, p.N - first) * groups / 8;
+    const __nv_bfloat16* s = p.sw + static_cast<int64_t>(first) * groups;     // one contiguous block
+    for (int c = threadIdx.x; c < n; c += blockDim.x) cp_async16(smem_u32(scales) + c * 16, s + c * 8, 16);
+  }
+  cp_async_commit();
+
+  const int64_t row_bytes = p.K >> 1;
+  const uint8_t* src = p.wq + (n0 + r) * row_bytes + q * 16;   // this lane's 16 bytes of channel r in the next group
+  int todo = live ? groups : 0;                                // groups still to request
+  uint32_t in = 0, out = 0;                                    // ring slots of the next request and the next entry
+  auto request = [&]() {
+#pragma unroll
+    for (int h = 0; h < GP; ++h) {
+      if (todo > h) {
+#pragma unroll
+        for (int c = 0; c < CT; ++c) cp_async16(ring + in + (h * CT + c) * 512, src + h * 64 + c * 8 * row_bytes, 16);
+      }
+    }
+    todo -= GP;
+    src += GP * 64;
+    in = in == (RING - 1) * kEntry ? 0u : in + kEntry;
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < RING - 1; ++i) request();
+  cp_async_wait<RING - 1>();
+  deal_tokens(p, xs, 0);
+  __syncthreads();
+
+  int xoff[MH];                                                // this lane's place in the tokens
+#pragma unroll
+  for (int t = 0; t < MH; ++t) {
+    const int tok = t * 8 + r;                                 // rows past M: any row, the result is not kept
+    xoff[t] = (tok < p.M ? tok : p.M - 1) * (p.chunk * 128 + 16) + q * 32;
+  }
+  float run[MT][CT][4] = {};
+  const __nv_bfloat16* sg = reinterpret_cast<const __nv_bfloat16*>(scales) + (warp * 8 * CT + 2 * q) * groups;
+  for (int g0 = 0; g0 < groups; g0 += p.chunk) {
+    if (g0 > 0) {                                              // the whole CTA: the next tokens
+      __syncthreads();
+      request_tokens(p, smem_u32(xs), g0);
+      cp_async_commit();
+      cp_async_wait<0>();
+      deal_tokens(p, xs, g0);
+      __syncthreads();
+    }
+    if (!live) continue;
+    const int n = min(groups - g0, p.chunk);
+    const uint8_t* xg = xs;
+    for (int g = 0; g < n; g += GP, xg += GP * 128) {
+      cp_async_wait<RING - 2>();
+      uint4 wv[GP][CT];
+#pragma unroll
+      for (int h = 0; h < GP; ++h)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) wv[h][c] = lds16(ring + out + (h * CT + c) * 512);
+      out = out == (RING - 1) * kEntry ? 0u : out + kEntry;
+      int acc[GP][MT][CT][4];
+#pragma unroll
+      for (int h = 0; h < GP; ++h) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int c = 0; c < CT; ++c) acc[h][t][c][0] = acc[h][t][c][1] = acc[h][t][c][2] = acc[h][t][c][3] = 0;
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {                       // 64 of the group's codes: two words of each lane
+          uint4 x[2 * MT];
+#pragma unroll
+          for (int t = 0; t < 2 * MT; ++t)
+            x[t] = t < MH ? *reinterpret_cast<const uint4*>(xg + h * 128 + xoff[t < MH ? t : 0] + jj * 16) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+              const uint4 v = wv[h][c];
+              const uint32_t word = jj ? (j ? v.w : v.z) : (j ? v.y : v.x);
+              const uint32_t b0 = (word << 4) & 0xF0F0F0F0u, b1 = word & 0xF0F0F0F0u;
+#pragma unroll
+              for (int t = 0; t < MT; ++t)
+                mma_s8_16832(acc[h][t][c], j ? x[2 * t].z : x[2 * t].x, j ? x[2 * t + 1].z : x[2 * t + 1].x,
+                             j ? x[2 * t].w : x[2 * t].y, j ? x[2 * t + 1].w : x[2 * t + 1].y, b0, b1);
+            }
+          }
+        }
+      }
+      request();
+#pragma unroll
+      for (int h = 0; h < GP; ++h) {
+        if (g + h < n) {
+#pragma unroll
+          for (int c = 0; c < CT; ++c) {
+            // the group sums hold 16 times the codes' product
+            const float s0 = __bfloat162float(sg[c * 8 * groups]) * 0.0625f, s1 = __bfloat162float(sg[(c * 8 + 1) * groups]) * 0.0625f;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+              run[t][c][0] = fmaf(static_cast<float>(acc[h][t][c][0]), s0, run[t][c][0]);
+              run[t][c][1] = fmaf(static_cast<float>(acc[h][t][c][1]), s1, run[t][c][1]);
+              if (2 * t + 1 < MH) {
+                run[t][c][2] = fmaf(static_cast<float>(acc[h][t][c][2]), s0, run[t][c][2]);
+                run[t][c][3] = fmaf(static_cast<float>(acc[h][t][c][3]), s1, run[t][c][3]);
+              }
+            }
+          }
+          ++sg;
+        }
+      }
     }
   }
-  if (lane < p.M) finish(p, lane, n, run);
+  if (!live) return;
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int m = t * 16 + r + 8 * (e >> 1), n = n0 + c * 8 + 2 * q + (e & 1);
+        if (m < p.M) finish(p, m, n, run[t][c][e]);
+      }
+}
+
+template <int MH, int CT, int GP, int RING>
+int launch_one(GemvParams p, int warps, cudaStream_t stream) {
+  const int tiles = p.N / (8 * CT), groups = p.K >> 7;
+  const int fixed = warps * (RING * CT * GP * 512 + groups * 16 * CT);
+  const int chunk = ((kSmemMax - fixed) / p.M - 16) / 128 / GP * GP;
+  if (fixed >= kSmemMax || chunk < GP) return fail(K2Q_EINVAL, "k2q_gemv_w4a8: no room for the tokens (M=%d, K=%d)", p.M, p.K);
+  p.chunk = chunk < groups ? chunk : (groups + GP - 1) / GP * GP;
+  const int smem = fixed + p.M * (p.chunk * 128 + 16);
+  auto kern = gemv_kernel<MH, CT, GP, RING>;
+  if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                          "cudaFuncSetAttribute(gemv_w4a8)"))
+    return rc;
+  p.warps = warps;
+  const int all = warps > 8 ? warps : 8;                       // eight warps at least stage the tokens
+  return launch_overlapped(kern, static_cast<unsigned>((tiles + warps - 1) / warps), static_cast<unsigned>(all * 32),
+                           static_cast<size_t>(smem), stream, 1, "gemv_w4a8 launch", p);
+}
+
+// One CTA per SM, as many warps as it takes to cover the channels at once (16 at most); where eight tiles of 16
+// channels and more fall to an SM, a warp takes 16, so that two of its channels share each read of the tokens.
+template <int MH>
+int launch_gemv(const GemvParams& p, cudaStream_t stream) {
+  const int sms = sm_count() > 0 ? sm_count() : 148, groups = p.K >> 7;
+  const int ct = p.N / 16 >= sms * 8 ? 2 : 1;
+  const int tiles = p.N / (8 * ct);
+  int warps = (tiles + sms - 1) / sms;
+  if (warps > kMaxWarps) warps = kMaxWarps;
+  const int room = 64 * 1024 / (groups * 16 * ct);             // the scales stay in shared memory
+  if (warps > room) warps = room;
+  if (ct == 2) return launch_one<MH, 2, 2, MH == 1 ? 4 : 3>(p, warps, stream);
+  return warps <= 8 ? launch_one<MH, 1, 4, 6>(p, warps, stream) : launch_one<MH, 1, 4, 4>(p, warps, stream);
 }
 
 }  // namespace
@@ -74,15 +279,15 @@ extern "C" int k2q_gemv_w4a8(const int8_t* xq, const uint8_t* wq4, const void* s
                              const k2q_epilogue* ep, void* y_bf16, int64_t ldy, void* stream) {
   const char* name = "k2q_gemv_w4a8";
   if (int rc = check_device_arch()) return rc;
-  if (M < 0 || M > kMaxRows || N <= 0 || K <= 0 || N > 0x7fffff00LL || K > 0x7fffff00LL)
-    return fail(K2Q_EINVAL, "%s: bad shape M=%lld N=%lld K=%lld (at most %d rows)", name, (long long)M, (long long)N,
-                (long long)K, kMaxRows);
+  if (M < 0 || M > kMaxRows || N <= 0 || K <= 0 || N > 0x7fffff00LL || K > kMaxK)
+    return fail(K2Q_EINVAL, "%s: bad shape M=%lld N=%lld K=%lld (at most %d rows, K <= %d)", name, (long long)M, (long long)N,
+                (long long)K, kMaxRows, kMaxK);
   if (K % 128 != 0) return fail(K2Q_EINVAL, "%s: K=%lld is not a multiple of 128", name, (long long)K);
   if (N % 16 != 0) return fail(K2Q_EINVAL, "%s: N=%lld is not a multiple of 16", name, (long long)N);
   if (M == 0) return K2Q_OK;
   if (!xq || !wq4 || !sw4_bf16 || !y_bf16) return fail(K2Q_EINVAL, "%s: NULL operand", name);
-  if ((reinterpret_cast<uintptr_t>(xq) | reinterpret_cast<uintptr_t>(wq4)) & 15u)
-    return fail(K2Q_EINVAL, "%s: codes must be 16-byte aligned", name);
+  if ((reinterpret_cast<uintptr_t>(xq) | reinterpret_cast<uintptr_t>(wq4) | reinterpret_cast<uintptr_t>(sw4_bf16)) & 15u)
+    return fail(K2Q_EINVAL, "%s: codes and group scales must be 16-byte aligned", name);
   if (ldy < N) return fail(K2Q_EINVAL, "%s: ldy < N", name);
   k2q_epilogue e{};
   if (ep) e = *ep;
@@ -97,6 +302,8 @@ extern "C" int k2q_gemv_w4a8(const int8_t* xq, const uint8_t* wq4, const void* s
   p.sx = e.sx; p.bias = e.bias; p.u = e.u; p.Bm = e.Bm; p.ldu = e.ldu; p.ldb = e.ldb; p.rank = e.rank;
   p.lora_scale = e.lora_scale; p.act = e.act;
   p.y = static_cast<__nv_bfloat16*>(y_bf16); p.ldy = ldy;
-  gemv_kernel<<<(p.N + kWarps - 1) / kWarps, kWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  return check_cuda(cudaGetLastError(), "gemv_w4a8 launch");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (M <= 8) return launch_gemv<1>(p, s);
+  if (M <= 16) return launch_gemv<2>(p, s);
+  return launch_gemv<4>(p, s);
 }

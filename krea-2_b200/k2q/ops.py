@@ -496,9 +496,12 @@ def _check_w4a8(name, xq, sx, wq4, sw4, bias, u, bm):
 
 def gemm_w4a8(xq, sx, wq4, sw4, bias=None, u=None, bm=None, lora_scale: float = 0.0, act=None,
               out: torch.Tensor | None = None) -> torch.Tensor:
-    """W4A8 variant: wq4 [N,K/2] packed uint8, sw4 [N,K/128] bf16."""
+    """W4A8 variant: wq4 [N,K/2] packed uint8, sw4 [N,K/128] bf16.  Up to ``GEMV_BEST_ROWS`` token rows go to
+    :func:`gemv_w4a8`: the same bits sooner."""
     dev = _need_cuda(xq, sx, wq4, sw4, bias, u, bm)
     m, n, k = _check_w4a8("gemm_w4a8", xq, sx, wq4, sw4, bias, u, bm)
+    if m <= GEMV_BEST_ROWS and n % 16 == 0 and k <= GEMV_MAX_K and xq.data_ptr() % 16 == 0 and wq4.data_ptr() % 16 == 0:
+        return gemv_w4a8(xq, sx, wq4, sw4, bias, u, bm, lora_scale, act, out)
     if out is not None:
         _check_out("gemm_w4a8", out, m, n, dev)
     y = out if out is not None else torch.empty(m, n, dtype=torch.bfloat16, device=dev)
@@ -511,6 +514,12 @@ def gemm_w4a8(xq, sx, wq4, sw4, bias=None, u=None, bm=None, lora_scale: float = 
 
 
 GEMV_ROWS = 32        # token rows that gemv_w4a8 takes
+GEMV_MAX_K = 131072
+# Rows that gemm_w4a8 hands to it.  Measured on a B200 with weights from DRAM, few-row kernel against the large
+# product's: 16 rows 27.0 / 68.8 us at 36864 x 6144, 12.6 / 27.6 at 6144 x 6144, 18.4 / 37.0 at 16384 x 6144, 3.8 / 5.8
+# at 6144 x 256; 32 rows 42.6 / 52.5, 20.2 / 27.3, 29.4 / 28.0, 5.3 / 5.8 -- between the two the large product's tiles
+# start to fill the SMs, and the few-row kernel's token reads to cost as much as the codes.
+GEMV_BEST_ROWS = 16
 
 
 def gemv_w4a8(xq, sx, wq4, sw4, bias=None, u=None, bm=None, lora_scale: float = 0.0, act=None,
@@ -527,6 +536,8 @@ def gemv_w4a8(xq, sx, wq4, sw4, bias=None, u=None, bm=None, lora_scale: float = 
     y = out if out is not None else torch.empty(m, n, dtype=torch.bfloat16, device=dev)
     if m == 0:
         return y
+    if sw4.data_ptr() % 16:
+        sw4 = sw4.clone()
     ep = _epilogue(sx, bias, u, bm, lora_scale, act)
     with torch.cuda.device(dev):
         rc = _lib.load().k2q_gemv_w4a8(_ptr(xq), _ptr(wq4), _ptr(sw4), m, n, k, C.byref(ep), _ptr(y),
