@@ -12,11 +12,13 @@
 //   gram    m' and the partial Gram matrices of pieces of the long side       12 B and S/2 FMA per element
 //   poly    partials added, normalised, iterated; leaves P = (Q ... Q_0) / (||u||_F + eps)
 //   apply   P u and the parameter step                                        16 B and S FMA per element
-// gram and apply are bound by HBM up to S = 32 and by the fp32 pipe beyond.  Both keep a sub-block of 2048 elements in
-// shared memory as it lies in memory, work on 4 x 4 register tiles with 16-byte shared reads (rows interleaved
-// over the tiles and a row pitch that is an odd number of 16-byte pieces, so that eight lanes meet eight
-// different pieces), and have the next sub-block in registers meanwhile.
-// The S x S iteration is in 64 bits: P's entries reach a^steps, so what G_0 loses to rounding comes back up to
+// gram and apply are bound by HBM up to S = 32 and by the fp32 pipe beyond.  Both work on sub-blocks of 4096 elements in
+// shared memory with 4 x 4 register tiles and packed fp32 pairs: a pair holds two neighbouring positions of the
+// CONTRACTED index, so no operand has to be broadcast and one instruction does two multiply-adds.  Where that index
+// is the contiguous one in memory (gram of a wide matrix, apply of a tall one) the sub-block stays as it is
+// ("natural"), otherwise neighbouring rows are interleaved on the way in ("paired").  The next sub-block travels
+// meanwhile by asynchronous copies into a raw area where every thread reads back only what it copied itself.
+// The S x S iteration is in 64 bits, on the fp64 tensor instructions (8 x 8 tiles of the upper triangle): P's entries reach a^steps, so what G_0 loses to rounding comes back up to
 // that much larger in the weak directions.  G_0's products are summed in fp32 by each thread over its share of a piece
 // (a few hundred terms), over threads in fp32, over pieces in 64 bits.  All sums run in a fixed order.
 #include "k2q_common.cuh"
@@ -26,7 +28,7 @@ namespace {
 
 constexpr int kMaxShort = 64;
 constexpr int kThreads = 256;
-constexpr int kVecs = 2;                       // 16-byte pieces of a sub-block per thread
+constexpr int kUnits = 2;                      // two rows by four columns of a sub-block, per thread
 constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;
 
 struct Mat {            // one entry of the device table
@@ -53,64 +55,53 @@ struct StepParams {
 __host__ __device__ constexpr int up4(int s) { return (s + 3) & ~3; }
 // 4 x 4 tiles of the upper triangle of a Gram matrix
 __host__ __device__ constexpr int pairs_of(int s) { return (up4(s) / 4) * (up4(s) / 4 + 1) / 2; }
-// positions of the long side per sub-block: 2048 elements, at least 32, a power of two
-__host__ __device__ constexpr int block_of(int s) { return s <= 4 ? 512 : s <= 8 ? 256 : s <= 16 ? 128 : s <= 32 ? 64 : 32; }
+// positions of the long side per sub-block: up to 4096 elements, a power of two
+__host__ __device__ constexpr int block_of(int s) { return s <= 4 ? 1024 : s <= 8 ? 512 : s <= 16 ? 256 : s <= 32 ? 128 : 64; }
+__host__ __device__ constexpr int odd_pitch(int w) { return ((w >> 2) & 1) ? w : w + 4; }
 
 __device__ __forceinline__ float clip_factor(const StepParams& a) {
   if (a.normsq == nullptr || !(a.max_norm > 0.f)) return 1.0f;
   return fminf(1.0f, a.max_norm / (sqrtf(__ldg(a.normsq)) + 1e-6f));
 }
 
-// A matrix as a CTA sees it: the sub-block is rows x width elements as stored (wide: S x block, tall: block x S).
+// A matrix as a CTA sees it: the sub-block is rows x width elements as stored (wide: S4 x block, tall: block x S4).
+// In shared memory
+//   natural   row r at r * pitch; the pitch is an odd number of 16-byte pieces, so that eight lanes on eight rows meet
+//             eight different pieces
+//   paired    rows 2r and 2r + 1 together at r * 2 * width: element pairs of columns 4c, 4c + 1 at 4c, those of columns
+//             4c + 2, 4c + 3 at width + 4c
 struct Place {
-  int s, s4, tall, block, width, pitch;
+  int s, s4, tall, block, width, rows, pitch;
   int64_t row_stride, step;                    // elements from row to row, from sub-block to sub-block
   bool vec;                                    // 16-byte accesses fit
   __device__ __forceinline__ Place(const Mat& t, int aligned) {
     s = t.s; s4 = up4(s); tall = t.tall; block = block_of(s);
     width = tall ? s4 : block;
-    pitch = ((width >> 2) & 1) ? width : width + 4;
+    rows = tall ? block : s4;
+    pitch = odd_pitch(width);
     row_stride = tall ? s : t.l;
     step = tall ? static_cast<int64_t>(block) * s : block;
     vec = aligned && (t.off & 3) == 0 && ((tall ? static_cast<int64_t>(s) : t.l) & 3) == 0;
   }
-};
-
-__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-
-// The thread's share of a sub-block in registers: kVecs pieces of four elements (element e of piece k).
-struct Share {
-  int64_t at[kVecs];    // offset of the piece in the matrix, sub-block 0
-  int sm[kVecs];        // place in shared memory
-  int lrel[kVecs];      // its (first) position along the long side within the sub-block
-  bool ok[kVecs];       // inside the sub-block
-  __device__ __forceinline__ Share(const Place& pl) {
-    const int per_row = pl.width >> 2, rows = pl.tall ? pl.block : pl.s;
-#pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
-      const int e = threadIdx.x + k * kThreads, r = e / per_row, c = (e - r * per_row) * 4;
-      ok[k] = r < rows;
-      at[k] = r * pl.row_stride + c;
-      sm[k] = r * pl.pitch + c;
-      lrel[k] = pl.tall ? r : c;
-    }
+  // elements of the four at (row, col .. col + 3) that exist, `left` positions of the long side remaining
+  __device__ __forceinline__ int len(int row, int col, int left) const {
+    const bool in = tall ? row < left : row < s;
+    return in ? max(0, min(4, (tall ? s : left) - col)) : 0;
   }
 };
 
-// Elements of a piece that exist: 4, or fewer at the end of a row or of the long side.
-__device__ __forceinline__ int piece_len(const Place& pl, const Share& sh, int k, int left) {
-  if (!sh.ok[k]) return 0;
-  if (pl.tall) return sh.lrel[k] < left ? min(4, pl.s - (sh.sm[k] - (sh.lrel[k] * pl.pitch))) : 0;
-  return max(0, min(4, left - sh.lrel[k]));
-}
-__device__ __forceinline__ float4 load_piece(const float* base, int n, bool vec) {
-  if (vec && n == 4) return ld4(base);
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (n > 0) v.x = base[0];
-  if (n > 1) v.y = base[1];
-  if (n > 2) v.z = base[2];
-  if (n > 3) v.w = base[3];
-  return v;
+__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ ulonglong2 ldp(const float* p) { return *reinterpret_cast<const ulonglong2*>(p); }
+
+// Requests four elements at base (n of them exist, the others become zero) into 16 bytes of shared memory.
+__device__ __forceinline__ void copy_piece(uint32_t dst, const float* base, int n, bool vec) {
+  if (vec) {
+    cp_async16(dst, base, n == 4 ? 16u : 0u);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * e), "l"(e < n ? base + e : base), "r"(e < n ? 4 : 0) : "memory");
+  }
 }
 __device__ __forceinline__ void store_piece(float* base, const float4& v, int n, bool vec) {
   if (vec && n == 4) {
@@ -122,6 +113,39 @@ __device__ __forceinline__ void store_piece(float* base, const float4& v, int n,
   if (n > 2) base[2] = v.z;
   if (n > 3) base[3] = v.w;
 }
+
+// The thread's share of a sub-block: kUnits times the same four columns of two neighbouring rows.
+// Piece k of it is row row[k / 2] + k % 2.
+struct Share {
+  int row[kUnits], col[kUnits];
+  int64_t at[kUnits];                          // offset of piece 2k; piece 2k + 1 is one row further
+  bool ok[kUnits];
+  bool full[2 * kUnits];                       // the piece exists whole in a sub-block that is whole (16-byte accesses)
+  __device__ __forceinline__ Share(const Place& pl) {
+    const int per_row = pl.width >> 2;
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      const int e = threadIdx.x + k * kThreads, r = e / per_row;
+      row[k] = 2 * r;
+      col[k] = (e - r * per_row) * 4;
+      ok[k] = 2 * r < pl.rows;
+      at[k] = row[k] * pl.row_stride + col[k];
+      full[2 * k] = ok[k] && pl.len(row[k], col[k], pl.block) == 4;
+      full[2 * k + 1] = ok[k] && pl.len(row[k] + 1, col[k], pl.block) == 4;
+    }
+  }
+  __device__ __forceinline__ void store_natural(float* u, const Place& pl, int k, const float4& a, const float4& b) const {
+    if (!ok[k]) return;
+    *reinterpret_cast<float4*>(u + row[k] * pl.pitch + col[k]) = a;
+    *reinterpret_cast<float4*>(u + (row[k] + 1) * pl.pitch + col[k]) = b;
+  }
+  __device__ __forceinline__ void store_paired(float* u, const Place& pl, int k, const float4& a, const float4& b) const {
+    if (!ok[k]) return;
+    float* at = u + row[k] * pl.width + col[k];
+    *reinterpret_cast<float4*>(at) = make_float4(a.x, b.x, a.y, b.y);
+    *reinterpret_cast<float4*>(at + pl.width) = make_float4(a.z, b.z, a.w, b.w);
+  }
+};
 // m' (in place) and u of four elements
 __device__ __forceinline__ float4 momentum4(const StepParams& a, float4 g, float4& m, float clip) {
   const float b = a.beta, c = 1.0f - a.beta;
@@ -137,22 +161,26 @@ __device__ __forceinline__ float4 update4(const StepParams& a, const float4& g, 
   return make_float4(b * m.x + c * (g.x * clip), b * m.y + c * (g.y * clip), b * m.z + c * (g.z * clip), b * m.w + c * (g.w * clip));
 }
 
-__host__ __device__ constexpr int sub_floats(int s, bool tall) {
-  const int w = tall ? up4(s) : block_of(s), p = ((w >> 2) & 1) ? w : w + 4;
-  return p * (tall ? block_of(s) : up4(s));
-}
 constexpr int max_sub_floats() {
   int best = 0;
   for (int s = 1; s <= kMaxShort; ++s) {
-    if (sub_floats(s, false) > best) best = sub_floats(s, false);
-    if (sub_floats(s, true) > best) best = sub_floats(s, true);
+    const int wide = up4(s) * odd_pitch(block_of(s)), tall = block_of(s) * odd_pitch(up4(s));
+    if (wide > best) best = wide;
+    if (tall > best) best = tall;
   }
   return best;
 }
 constexpr int kMaxSub = max_sub_floats();
+static_assert(kThreads * 16 <= kMaxSub, "the gram kernel adds its threads' shares in the sub-block's place");
 
-__global__ void __launch_bounds__(kThreads) gram_kernel(const StepParams a) {
-  __shared__ __align__(16) float u[kMaxSub > kThreads * 16 ? kMaxSub : kThreads * 16];
+constexpr int kRaw = 2 * kUnits * kThreads * 16;               // bytes of one buffer's raw sub-block
+constexpr int kGramSmem = 2 * kRaw + kMaxSub * 4;
+
+__global__ void __launch_bounds__(kThreads, 3) gram_kernel(const StepParams a) {
+  extern __shared__ __align__(16) float smem[];
+  float* u = smem;
+  float* raw = smem + kMaxSub + threadIdx.x * 4;               // piece k of this thread: g at k, m at 2 * kUnits + k
+  const uint32_t raw_u32 = smem_u32(raw);
   const Tile tile = a.tiles[blockIdx.x];
   const Mat t = a.mats[tile.mat];
   const Place pl(t, a.aligned);
@@ -161,71 +189,103 @@ __global__ void __launch_bounds__(kThreads) gram_kernel(const StepParams a) {
   const int64_t last = min(t.l, tile.first + a.piece);
   const int nt = pl.s4 >> 2, pairs = pairs_of(t.s), kgroups = kThreads / pairs;
   // this thread's tile (ti <= tj) and share of the positions
-  const int kg = threadIdx.x / pairs;
-  int ti = 0, tj = threadIdx.x - kg * pairs;
+  const int kg = threadIdx.x / pairs, mine = threadIdx.x - kg * pairs;
+  int ti = 0, tj = mine;
   while (tj >= nt - ti) { tj -= nt - ti; ++ti; }
   tj += ti;
   const bool works = kg < kgroups;
-  float acc[4][4] = {};
+  uint64_t acc[4][4] = {};                     // sums over the even and over the odd positions
 
-  const int64_t origin = t.off + (t.tall ? tile.first * t.s : tile.first);
-  float4 rg[kVecs], rm[kVecs];
-  int rn[kVecs];
-  int64_t base = origin;
-  auto fetch = [&](int64_t c0) {
-    const int left = static_cast<int>(min(static_cast<int64_t>(pl.block), last - c0));
+  int64_t base = t.off + (t.tall ? tile.first * t.s : tile.first);
+  const bool has_m = a.m != nullptr;
+  auto fetch = [&](int64_t at, int left) {
+    if (pl.vec && left == pl.block) {          // whole sub-block: what exists was settled beforehand
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
-      rn[k] = piece_len(pl, sh, k, left);
-      rg[k] = load_piece(a.g + base + sh.at[k], rn[k], pl.vec);
-      if (a.m != nullptr) rm[k] = load_piece(a.m + base + sh.at[k], rn[k], pl.vec);
-    }
-  };
-  // rows of the padding (wide: S .. S4) stay zero
-  for (int e = threadIdx.x; e < (pl.tall ? 0 : (pl.s4 - pl.s) * pl.pitch); e += kThreads) u[pl.s * pl.pitch + e] = 0.f;
-  fetch(tile.first);
-  for (int64_t c0 = tile.first; c0 < last; c0 += pl.block) {
-#pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
-      float4 v = rg[k];
-      if (a.m != nullptr) {
-        v = momentum4(a, rg[k], rm[k], clip);
-        store_piece(a.m + base + sh.at[k], rm[k], rn[k], pl.vec);
-        if (rn[k] < 4) {                       // positions that do not exist count as zero
-          if (rn[k] < 1) v.x = 0.f;
-          if (rn[k] < 2) v.y = 0.f;
-          if (rn[k] < 3) v.z = 0.f;
-          v.w = 0.f;
+      for (int k = 0; k < 2 * kUnits; ++k) {
+        const int64_t o = at + sh.at[k >> 1] + (k & 1) * pl.row_stride;
+        if (sh.full[k]) {
+          cp_async16(raw_u32 + k * (kThreads * 16), a.g + o, 16);
+          if (has_m) cp_async16(raw_u32 + kRaw + k * (kThreads * 16), a.m + o, 16);
         }
       }
-      if (sh.ok[k]) *reinterpret_cast<float4*>(u + sh.sm[k]) = v;
+    } else {
+#pragma unroll 1
+      for (int k = 0; k < 2 * kUnits; ++k) {
+        const int row = 2 * ((threadIdx.x + (k >> 1) * kThreads) / (pl.width >> 2)) + (k & 1);
+        const int col = (threadIdx.x + (k >> 1) * kThreads) % (pl.width >> 2) * 4;
+        const int n = row < pl.rows ? pl.len(row, col, left) : 0;
+        const int64_t o = n > 0 ? at + row * pl.row_stride + col : 0;
+        copy_piece(raw_u32 + k * (kThreads * 16), a.g + o, n, pl.vec);
+        if (has_m) copy_piece(raw_u32 + kRaw + k * (kThreads * 16), a.m + o, n, pl.vec);
+      }
+    }
+    cp_async_commit();
+  };
+  auto left_of = [&](int64_t c0) { return static_cast<int>(min(static_cast<int64_t>(pl.block), last - c0)); };
+#pragma unroll
+  for (int k = 0; k < 4 * kUnits; ++k) *reinterpret_cast<float4*>(raw + k * (kThreads * 4)) = make_float4(0.f, 0.f, 0.f, 0.f);
+  fetch(base, left_of(tile.first));
+  for (int64_t c0 = tile.first; c0 < last; c0 += pl.block) {
+    const int left = left_of(c0);
+    const bool whole = pl.vec && left == pl.block;
+    cp_async_wait<0>();
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      float4 v[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        v[h] = ld4(raw + (2 * k + h) * (kThreads * 4));
+        if (has_m) {
+          float4 m = ld4(raw + (2 * kUnits + 2 * k + h) * (kThreads * 4));
+          v[h] = momentum4(a, v[h], m, clip);
+          float* out = a.m + base + sh.at[k] + h * pl.row_stride;
+          if (whole) {
+            if (sh.full[2 * k + h]) *reinterpret_cast<float4*>(out) = m;
+            else v[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+          } else {
+            const int n = sh.ok[k] ? pl.len(sh.row[k] + h, sh.col[k], left) : 0;
+            store_piece(out, m, n, pl.vec);
+            if (n < 4) {                       // positions that do not exist count as zero, whatever the clip factor is
+              if (n < 1) v[h].x = 0.f;
+              if (n < 2) v[h].y = 0.f;
+              if (n < 3) v[h].z = 0.f;
+              v[h].w = 0.f;
+            }
+          }
+        }
+      }
+      if (pl.tall) sh.store_paired(u, pl, k, v[0], v[1]);
+      else sh.store_natural(u, pl, k, v[0], v[1]);
     }
     base += pl.step;
     __syncthreads();
-    if (c0 + pl.block < last) fetch(c0 + pl.block);
+    if (c0 + pl.block < last) fetch(base, left_of(c0 + pl.block));
     if (works) {
       if (pl.tall) {
-        for (int l = kg; l < pl.block; l += kgroups) {
-          const float4 x = ld4(u + l * pl.pitch + 4 * ti), y = ld4(u + l * pl.pitch + 4 * tj);
-          const float xv[4] = {x.x, x.y, x.z, x.w}, yv[4] = {y.x, y.y, y.z, y.w};
+        const float *xp = u + 4 * ti, *yp = u + 4 * tj;
+#pragma unroll 2
+        for (int l = kg; l < pl.block / 2; l += kgroups) {
+          const float *xr = xp + l * 2 * pl.width, *yr = yp + l * 2 * pl.width;
+          const ulonglong2 x0 = ldp(xr), x1 = ldp(xr + pl.width), y0 = ldp(yr), y1 = ldp(yr + pl.width);
+          const uint64_t x[4] = {x0.x, x0.y, x1.x, x1.y}, y[4] = {y0.x, y0.y, y1.x, y1.y};
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xv[i], yv[j], acc[i][j]);
+            for (int j = 0; j < 4; ++j) acc[i][j] = fma_f32x2(x[i], y[j], acc[i][j]);
         }
       } else {
+        const float *xp = u + ti * pl.pitch, *yp = u + tj * pl.pitch;
+        const int hop = nt * pl.pitch;
         for (int l = 4 * kg; l < pl.block; l += 4 * kgroups) {
-          float4 x[4], y[4];
+          ulonglong2 y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j] = ldp(yp + j * hop + l);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            x[i] = ld4(u + (ti + i * nt) * pl.pitch + l);
-            y[i] = ld4(u + (tj + i * nt) * pl.pitch + l);
+            const ulonglong2 x = ldp(xp + i * hop + l);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = fma_f32x2(x.y, y[j].y, fma_f32x2(x.x, y[j].x, acc[i][j]));
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              acc[i][j] = fmaf(x[i].w, y[j].w, fmaf(x[i].z, y[j].z, fmaf(x[i].y, y[j].y, fmaf(x[i].x, y[j].x, acc[i][j]))));
         }
       }
     }
@@ -236,7 +296,11 @@ __global__ void __launch_bounds__(kThreads) gram_kernel(const StepParams a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u[(kg * 16 + i * 4 + j) * pairs + (threadIdx.x - kg * pairs)] = acc[i][j];
+      for (int j = 0; j < 4; ++j) {
+        float lo, hi;
+        unpack_f32x2(acc[i][j], lo, hi);
+        u[(kg * 16 + i * 4 + j) * pairs + mine] = lo + hi;
+      }
   }
   __syncthreads();
   float* part = a.ws + t.gram + static_cast<int64_t>(blockIdx.x - t.tile0) * pairs * 16;
@@ -247,23 +311,53 @@ __global__ void __launch_bounds__(kThreads) gram_kernel(const StepParams a) {
   }
 }
 
-// d = x y for S4 x S4 matrices (padding rows and columns are zero), 4 x 2 register tiles
-__device__ __forceinline__ void matmul(double* d, const double* x, const double* y, int s4) {
-  const int across = s4 >> 1, tiles = (s4 >> 2) * across;
-  for (int e = threadIdx.x; e < tiles; e += kThreads) {
-    const int i = e / across * 4, j = (e - e / across * across) * 2;
-    double v[4][2] = {};
-    for (int k = 0; k < s4; ++k) {
-      const double2 b = *reinterpret_cast<const double2*>(y + k * s4 + j);
+// S x S matrices of the iteration in shared memory: S8 rows, the padding zero; the pitch lets the 32 lanes of a
+// fragment read (8 rows, 4 neighbours each) meet all banks.
+__host__ __device__ constexpr int up8(int s) { return (s + 7) & ~7; }
+__host__ __device__ constexpr int pitch64(int s) { return ((s + 15) & ~15) + 4; }
+
+// For two commuting symmetric matrices: d = alpha I + beta y + gamma x y on the upper triangle and mirrored (alpha on the
+// first s entries of the diagonal).  A warp takes every eighth 8 x 8 tile.  x y is symmetric up to rounding in 64 bits,
+// so y's columns may be read as its rows.
+__device__ __forceinline__ void poly_step(double* d, const double* x, const double* y, int s, double alpha, double beta, double gamma) {
+  const int n8 = up8(s) >> 3, pitch = pitch64(s), lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
+  const int pairs = n8 * (n8 + 1) / 2;
+  constexpr int kWarps = kThreads / 32;
+  for (int e0 = threadIdx.x >> 5; e0 < pairs; e0 += 2 * kWarps) {      // two tiles at a time, two sums each: four chains
+    int it[2], jt[2];
+    double c[2][2][2] = {};
+    const double *xa[2], *yb[2];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const double c = x[(i + r) * s4 + k];
-        v[r][0] = fma(c, b.x, v[r][0]);
-        v[r][1] = fma(c, b.y, v[r][1]);
-      }
+    for (int w = 0; w < 2; ++w) {
+      int ti = 0, tj = e0 + w * kWarps < pairs ? e0 + w * kWarps : e0;   // past the end: the first once more, not stored
+      while (tj >= n8 - ti) { tj -= n8 - ti; ++ti; }
+      tj += ti;
+      it[w] = 8 * ti + r;
+      jt[w] = 8 * tj + 2 * q;
+      xa[w] = x + (8 * ti + r) * pitch + q;
+      yb[w] = y + (8 * tj + r) * pitch + q;
     }
+#pragma unroll 2
+    for (int k = 0; k < 8 * n8; k += 8)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) *reinterpret_cast<double2*>(d + (i + r) * s4 + j) = make_double2(v[r][0], v[r][1]);
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+          asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};"
+              : "+d"(c[w][h][0]), "+d"(c[w][h][1])
+              : "d"(xa[w][k + 4 * h]), "d"(yb[w][k + 4 * h]));
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      if (e0 + w * kWarps >= pairs) break;
+      const int i = it[w], j = jt[w];
+      double c0 = gamma * (c[w][0][0] + c[w][1][0]), c1 = gamma * (c[w][0][1] + c[w][1][1]);
+      if (beta != 0.0) {
+        c0 += beta * y[i * pitch + j] + (i == j && i < s ? alpha : 0.0);
+        c1 += beta * y[i * pitch + j + 1] + (i == j + 1 && i < s ? alpha : 0.0);
+      }
+      if (i <= j) d[i * pitch + j] = d[j * pitch + i] = c0;      // one writer per entry, in diagonal tiles too
+      if (i <= j + 1) d[i * pitch + j + 1] = d[(j + 1) * pitch + i] = c1;
+    }
   }
   __syncthreads();
 }
@@ -272,8 +366,10 @@ __global__ void __launch_bounds__(kThreads) poly_kernel(const StepParams a) {
   extern __shared__ __align__(16) double sh[];
   __shared__ double inv;
   const Mat t = a.mats[blockIdx.x];
-  const int s4 = up4(t.s), n = s4 * s4, nt = s4 >> 2, pairs = pairs_of(t.s);
+  const int s4 = up4(t.s), nt = s4 >> 2, pairs = pairs_of(t.s), pitch = pitch64(t.s), n = up8(t.s) * pitch;
   double *g = sh, *q = sh + n, *x = sh + 2 * n, *y = sh + 3 * n;
+  for (int e = threadIdx.x; e < n; e += kThreads) g[e] = 0.0;
+  __syncthreads();
   for (int e = threadIdx.x; e < pairs * 16; e += kThreads) {
     double v = 0.0;
     const float* part = a.ws + t.gram + e;
@@ -285,46 +381,40 @@ __global__ void __launch_bounds__(kThreads) poly_kernel(const StepParams a) {
     tj += ti;
     // rows of a tile: neighbours where the matrix is tall, every nt-th where it is wide
     const int i = t.tall ? 4 * ti + (in >> 2) : ti + (in >> 2) * nt, j = t.tall ? 4 * tj + (in & 3) : tj + (in & 3) * nt;
-    g[i * s4 + j] = v;
-    g[j * s4 + i] = v;
+    g[i * pitch + j] = v;
+    g[j * pitch + i] = v;
   }
   __syncthreads();
   if (threadIdx.x < 32) {
     double tr = 0.0;
-    for (int i = threadIdx.x; i < s4; i += 32) tr += g[i * s4 + i];
+    for (int i = threadIdx.x; i < t.s; i += 32) tr += g[i * pitch + i];
     for (int o = 16; o > 0; o >>= 1) tr += __shfl_xor_sync(0xffffffffu, tr, o);
     if (threadIdx.x == 0) inv = 1.0 / (sqrt(tr) + static_cast<double>(a.eps));
   }
   __syncthreads();
   const double f = inv;
   for (int e = threadIdx.x; e < n; e += kThreads) {
-    const bool diag = e / s4 == e % s4 && e / s4 < t.s;
     g[e] *= f * f;
-    if (a.steps == 0) x[e] = diag ? 1.0 : 0.0;
+    if (a.steps == 0) x[e] = e / pitch == e % pitch ? 1.0 : 0.0;
   }
   __syncthreads();
   for (int it = 0; it < a.steps; ++it) {
-    double* dst = it == 0 ? x : q;             // the first factor is the product so far
-    matmul(dst, g, g, s4);
-    for (int e = threadIdx.x; e < n; e += kThreads) {
-      const bool diag = e / s4 == e % s4 && e / s4 < t.s;
-      dst[e] = (diag ? kA : 0.0) + kB * g[e] + kC * dst[e];
-    }
-    __syncthreads();
+    double* factor = it == 0 ? x : q;          // the first factor is the product so far
+    poly_step(factor, g, g, t.s, kA, kB, kC);
     if (it > 0) {
-      matmul(y, q, x, s4);
+      poly_step(y, q, x, t.s, 0.0, 0.0, 1.0);
       double* o = x; x = y; y = o;
     }
     if (it + 1 < a.steps) {
       const double* f1 = it == 0 ? x : q;
-      matmul(y, f1, g, s4);
-      matmul(g, f1, y, s4);
+      poly_step(y, f1, g, t.s, 0.0, 0.0, 1.0);
+      poly_step(g, f1, y, t.s, 0.0, 0.0, 1.0);
     }
   }
-  for (int e = threadIdx.x; e < n; e += kThreads) a.ws[t.poly + e] = static_cast<float>(x[e] * f);
+  for (int e = threadIdx.x; e < s4 * s4; e += kThreads) a.ws[t.poly + e] = static_cast<float>(x[e / s4 * pitch + e % s4] * f);
 }
 
-__global__ void __launch_bounds__(kThreads) apply_kernel(const StepParams a) {
+__global__ void __launch_bounds__(kThreads, 2) apply_kernel(const StepParams a) {
   extern __shared__ __align__(16) float smem[];
   const Tile tile = a.tiles[blockIdx.x];
   const Mat t = a.mats[tile.mat];
@@ -335,99 +425,139 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(const StepParams a) {
   const float rows = t.tall ? t.l : t.s, cols = t.tall ? t.s : t.l;
   const float step = a.lr * (a.scale_mode == 0 ? 0.2f * sqrtf(fmaxf(rows, cols)) : sqrtf(fmaxf(1.0f, rows / cols)));
   const float keep = 1.0f - a.lr * a.wd;
-  float* u = smem;                                             // sub-block, replaced by its product
-  float* pm = smem + kMaxSub;                         // P [S4][pp]
-  const int pp = ((pl.s4 >> 2) & 1) ? pl.s4 : pl.s4 + 4;
-  for (int e = threadIdx.x; e < pl.s4 * pl.s4; e += kThreads) pm[e / pl.s4 * pp + e % pl.s4] = a.ws[t.poly + e];
-  for (int e = threadIdx.x; e < (pl.tall ? 0 : (pl.s4 - pl.s) * pl.pitch); e += kThreads) u[pl.s * pl.pitch + e] = 0.f;
-
-  // out = A B with A's rows (wide: P, tall: the sub-block) interleaved over the tiles, B's columns neighbours
+  float* u = smem;
+  float* pm = smem + kMaxSub;                                  // P: natural where the matrix is wide, paired where it is tall
+  const int pp = odd_pitch(pl.s4);
+  for (int e = threadIdx.x; e < pl.s4 * pl.s4; e += kThreads) {
+    const int r = e / pl.s4, c = e - r * pl.s4;
+    const int at = pl.tall ? (r >> 1) * 2 * pl.s4 + ((c >> 1) & 1) * pl.s4 + (c & ~3) + (c & 1) * 2 + (r & 1) : r * pp + c;
+    pm[at] = a.ws[t.poly + e];
+  }
+  // out = A B: A (wide: P, tall: the sub-block) natural, its rows interleaved over the tiles; B paired
   const float *am = pl.tall ? u : pm, *bm = pl.tall ? pm : u;
-  const int ap = pl.tall ? pl.pitch : pp, bp = pl.tall ? pp : pl.pitch;
-  const int out_rows = pl.tall ? pl.block : pl.s4, rt = out_rows >> 2, ct = pl.width >> 2;
-  const int tiles = rt * ct;                                   // 2048 / 16: half of the threads multiply
+  const int ap = pl.tall ? pl.pitch : pp, bw = pl.tall ? pl.s4 : pl.width;
+  const int rt = pl.rows >> 2, ct = pl.width >> 2;             // up to 256 tiles of 4 x 4
+  const int ri = threadIdx.x / ct, ci = (threadIdx.x - ri * ct) * 4;
+  const bool works = ri < rt;
 
-  float4 rg[kVecs], rm[kVecs], rp[kVecs];
-  int rn[kVecs];
+  // raw pieces of this thread: g, m as the shares say, p where its results go
+  float* raw = pm + up4(kMaxShort) * odd_pitch(up4(kMaxShort)) + threadIdx.x * 4;
+  const uint32_t raw_u32 = smem_u32(raw);
   int64_t base = t.off + (t.tall ? tile.first * t.s : tile.first);
-  auto fetch = [&](int64_t c0) {
-    const int left = static_cast<int>(min(static_cast<int64_t>(pl.block), last - c0));
+  const bool want_g = a.m == nullptr || a.nesterov;
+  auto left_of = [&](int64_t c0) { return static_cast<int>(min(static_cast<int64_t>(pl.block), last - c0)); };
+  const bool has_m = a.m != nullptr, to_p = a.out == nullptr;
+  auto fetch = [&](int64_t at, int left) {
+    if (pl.vec && left == pl.block) {
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
-      rn[k] = piece_len(pl, sh, k, left);
-      if (a.m == nullptr || a.nesterov) rg[k] = load_piece(a.g + base + sh.at[k], rn[k], pl.vec);
-      if (a.m != nullptr) rm[k] = load_piece(a.m + base + sh.at[k], rn[k], pl.vec);
-      if (a.out == nullptr) rp[k] = load_piece(a.p + base + sh.at[k], rn[k], pl.vec);
+      for (int k = 0; k < 2 * kUnits; ++k) {
+        const int64_t o = at + sh.at[k >> 1] + (k & 1) * pl.row_stride;
+        if (sh.full[k]) {
+          if (want_g) cp_async16(raw_u32 + k * (kThreads * 16), a.g + o, 16);
+          if (has_m) cp_async16(raw_u32 + kRaw + k * (kThreads * 16), a.m + o, 16);
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int k = 0; k < 2 * kUnits; ++k) {
+        const int row = 2 * ((threadIdx.x + (k >> 1) * kThreads) / (pl.width >> 2)) + (k & 1);
+        const int col = (threadIdx.x + (k >> 1) * kThreads) % (pl.width >> 2) * 4;
+        const int n = row < pl.rows ? pl.len(row, col, left) : 0;
+        const int64_t o = n > 0 ? at + row * pl.row_stride + col : 0;
+        if (want_g) copy_piece(raw_u32 + k * (kThreads * 16), a.g + o, n, pl.vec);
+        if (has_m) copy_piece(raw_u32 + kRaw + k * (kThreads * 16), a.m + o, n, pl.vec);
+      }
     }
+    cp_async_commit();
   };
-  fetch(tile.first);
-  for (int64_t c0 = tile.first; c0 < last; c0 += pl.block) {
-    float4 cur_p[kVecs];
-    int cur_n[kVecs];
-    const int64_t cur = base;
-    __syncthreads();
+  const int64_t out_at = ri * pl.row_stride + ci, out_hop = rt * pl.row_stride;
+  auto fetch_p = [&](int64_t at, int left) {
+    if (to_p && works) {
+      if (pl.vec && left == pl.block) {
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
-      if (sh.ok[k]) *reinterpret_cast<float4*>(u + sh.sm[k]) = a.m == nullptr ? rg[k] : update4(a, rg[k], rm[k], clip);
-      cur_p[k] = rp[k];
-      cur_n[k] = rn[k];
+        for (int i = 0; i < 4; ++i)
+          if (pl.tall || ri + i * rt < pl.s) cp_async16(raw_u32 + 2 * kRaw + i * (kThreads * 16), a.p + at + out_at + i * out_hop, 16);
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          const int n = pl.len(ri + i * rt, ci, left);
+          copy_piece(raw_u32 + 2 * kRaw + i * (kThreads * 16), a.p + (n > 0 ? at + out_at + i * out_hop : 0), n, pl.vec);
+        }
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < 4 * kUnits; ++k) *reinterpret_cast<float4*>(raw + k * (kThreads * 4)) = make_float4(0.f, 0.f, 0.f, 0.f);
+  fetch(base, left_of(tile.first));
+  fetch_p(base, left_of(tile.first));
+  for (int64_t c0 = tile.first; c0 < last; c0 += pl.block) {
+    const int64_t cur = base;
+    const int left = left_of(c0);
+    const bool whole = pl.vec && left == pl.block;
+    cp_async_wait<1>();                                        // g and m; p is still on its way
+    __syncthreads();                                           // the sub-block before has been read (and P is in place)
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      float4 v[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 g4 = want_g ? ld4(raw + (2 * k + h) * (kThreads * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[h] = !has_m ? g4 : update4(a, g4, ld4(raw + (2 * kUnits + 2 * k + h) * (kThreads * 4)), clip);
+      }
+      if (pl.tall) sh.store_natural(u, pl, k, v[0], v[1]);
+      else sh.store_paired(u, pl, k, v[0], v[1]);
     }
     __syncthreads();
     base += pl.step;
-    if (c0 + pl.block < last) fetch(c0 + pl.block);
-    float acc[4][4];
-    int ri = 0, ci = 0;
-    const bool works = static_cast<int>(threadIdx.x) < tiles;
+    const int next = c0 + pl.block < last ? left_of(c0 + pl.block) : 0;
+    fetch(base, next);                                         // nothing exists past the end: no copy leaves
     if (works) {
-      ri = threadIdx.x / ct;
-      ci = (threadIdx.x - ri * ct) * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-      for (int k = 0; k < pl.s4; k += 4) {
-        float4 x[4], y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = ld4(am + (ri + i * rt) * ap + k);
-          y[i] = ld4(bm + (k + i) * bp + ci);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float xv[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            acc[i][0] = fmaf(xv[kk], y[kk].x, acc[i][0]);
-            acc[i][1] = fmaf(xv[kk], y[kk].y, acc[i][1]);
-            acc[i][2] = fmaf(xv[kk], y[kk].z, acc[i][2]);
-            acc[i][3] = fmaf(xv[kk], y[kk].w, acc[i][3]);
-          }
-        }
-      }
-    }
-    __syncthreads();
-    if (works) {
+    uint64_t acc[4][4] = {};
+    const float *ax = am + ri * ap, *by = bm + ci;
+    const int hop = rt * ap;
+    for (int k = 0; k < pl.s4; k += 4) {
+      const float* b0 = by + k * bw;
+      const ulonglong2 y00 = ldp(b0), y01 = ldp(b0 + bw), y10 = ldp(b0 + 2 * bw), y11 = ldp(b0 + 3 * bw);
+      const uint64_t ya[4] = {y00.x, y00.y, y01.x, y01.y}, yb[4] = {y10.x, y10.y, y11.x, y11.y};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int r = ri + i * rt;
-        if (pl.tall || r < pl.s) *reinterpret_cast<float4*>(u + r * pl.pitch + ci) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-      }
-    }
-    __syncthreads();
+        const ulonglong2 x = ldp(ax + i * hop + k);
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
-      if (!sh.ok[k]) continue;
-      float4 o = ld4(u + sh.sm[k]);
-      if (a.out != nullptr) {
-        store_piece(a.out + cur + sh.at[k], o, cur_n[k], pl.vec);
-      } else {
-        const float4 p0 = cur_p[k];
-        o.x = p0.x * keep - step * o.x; o.y = p0.y * keep - step * o.y;
-        o.z = p0.z * keep - step * o.z; o.w = p0.w * keep - step * o.w;
-        store_piece(a.p + cur + sh.at[k], o, cur_n[k], pl.vec);
-        if (a.zero_grad) store_piece(a.g + cur + sh.at[k], make_float4(0.f, 0.f, 0.f, 0.f), cur_n[k], pl.vec);
+        for (int j = 0; j < 4; ++j) acc[i][j] = fma_f32x2(x.y, yb[j], fma_f32x2(x.x, ya[j], acc[i][j]));
       }
     }
+    cp_async_wait<1>();                                        // p; the next g and m are on their way
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float lo, hi;
+        unpack_f32x2(acc[i][j], lo, hi);
+        o[j] = lo + hi;
+      }
+      const int64_t at = cur + out_at + i * out_hop;
+      float4 v = make_float4(o[0], o[1], o[2], o[3]);
+      if (to_p) {
+        const float4 p0 = ld4(raw + (4 * kUnits + i) * (kThreads * 4));
+        v = make_float4(p0.x * keep - step * o[0], p0.y * keep - step * o[1], p0.z * keep - step * o[2], p0.w * keep - step * o[3]);
+      }
+      float* out = (to_p ? a.p : a.out) + at;
+      // the gradients are zeroed by the CTA that alone reads them, after it has
+      if (whole) {
+        if (pl.tall || ri + i * rt < pl.s) {
+          *reinterpret_cast<float4*>(out) = v;
+          if (a.zero_grad) *reinterpret_cast<float4*>(a.g + at) = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      } else {
+        const int n = pl.len(ri + i * rt, ci, left);
+        store_piece(out, v, n, pl.vec);
+        if (a.zero_grad) store_piece(a.g + at, make_float4(0.f, 0.f, 0.f, 0.f), n, pl.vec);
+      }
+    }
+    }
+    fetch_p(base, next);
   }
 }
 
@@ -479,12 +609,19 @@ int run_steps(const char* name, const k2q_matrices* pl, const void* table, StepP
   a.ws = static_cast<float*>(ws);
   a.aligned = !off16(a.p) && !off16(a.g) && !off16(a.m) && !off16(a.out);
   const int s4 = up4(pl->max_short);
-  const int poly_smem = 4 * s4 * s4 * 8, apply_smem = (kMaxSub + s4 * (s4 + 4)) * 4;
+  const int poly_smem = 4 * up8(pl->max_short) * pitch64(pl->max_short) * 8;
+  const int apply_smem = (kMaxSub + up4(kMaxShort) * odd_pitch(up4(kMaxShort))) * 4 + 3 * kRaw;
+  if (int rc = check_cuda(cudaFuncSetAttribute(gram_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGramSmem),
+                          "cudaFuncSetAttribute(gram)"))
+    return rc;
   if (int rc = check_cuda(cudaFuncSetAttribute(poly_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, poly_smem),
                           "cudaFuncSetAttribute(poly)"))
     return rc;
+  if (int rc = check_cuda(cudaFuncSetAttribute(apply_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, apply_smem),
+                          "cudaFuncSetAttribute(apply)"))
+    return rc;
   const unsigned tiles = static_cast<unsigned>(pl->tiles);
-  gram_kernel<<<tiles, kThreads, 0, s>>>(a);
+  gram_kernel<<<tiles, kThreads, kGramSmem, s>>>(a);
   poly_kernel<<<static_cast<unsigned>(pl->count), kThreads, poly_smem, s>>>(a);
   apply_kernel<<<tiles, kThreads, apply_smem, s>>>(a);
   return check_cuda(cudaGetLastError(), name);
