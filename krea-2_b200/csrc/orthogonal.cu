@@ -74,8 +74,9 @@ struct Place {
   int s, s4, tall, block, width, rows, pitch;
   int64_t row_stride, step;                    // elements from row to row, from sub-block to sub-block
   bool vec;                                    // 16-byte accesses fit
-  __device__ __forceinline__ Place(const Mat& t, int aligned) {
-    s = t.s; s4 = up4(s); tall = t.tall; block = block_of(s);
+  // orientation and block come in as constants: the kernels' bodies are compiled for each
+  __device__ __forceinline__ Place(const Mat& t, int aligned, bool tall_, int block_) {
+    s = t.s; s4 = up4(s); tall = tall_; block = block_;
     width = tall ? s4 : block;
     rows = tall ? block : s4;
     pitch = odd_pitch(width);
@@ -176,14 +177,12 @@ static_assert(kThreads * 16 <= kMaxSub, "the gram kernel adds its threads' share
 constexpr int kRaw = 2 * kUnits * kThreads * 16;               // bytes of one buffer's raw sub-block
 constexpr int kGramSmem = 2 * kRaw + kMaxSub * 4;
 
-__global__ void __launch_bounds__(kThreads, 3) gram_kernel(const StepParams a) {
-  extern __shared__ __align__(16) float smem[];
+template <bool TALL, int BLOCK>
+__device__ __forceinline__ void gram_body(const StepParams& a, const Tile& tile, const Mat& t, float* smem) {
   float* u = smem;
   float* raw = smem + kMaxSub + threadIdx.x * 4;               // piece k of this thread: g at k, m at 2 * kUnits + k
   const uint32_t raw_u32 = smem_u32(raw);
-  const Tile tile = a.tiles[blockIdx.x];
-  const Mat t = a.mats[tile.mat];
-  const Place pl(t, a.aligned);
+  const Place pl(t, a.aligned, TALL, BLOCK);
   const Share sh(pl);
   const float clip = clip_factor(a);
   const int64_t last = min(t.l, tile.first + a.piece);
@@ -311,66 +310,112 @@ __global__ void __launch_bounds__(kThreads, 3) gram_kernel(const StepParams a) {
   }
 }
 
+#define K2Q_BY_SHAPE(body)                                              \
+  if (t.tall) {                                                         \
+    switch (block_of(t.s)) {                                            \
+      case 1024: body<true, 1024>(a, tile, t, smem); break;             \
+      case 512: body<true, 512>(a, tile, t, smem); break;               \
+      case 256: body<true, 256>(a, tile, t, smem); break;               \
+      case 128: body<true, 128>(a, tile, t, smem); break;               \
+      default: body<true, 64>(a, tile, t, smem); break;                 \
+    }                                                                   \
+  } else {                                                              \
+    switch (block_of(t.s)) {                                            \
+      case 1024: body<false, 1024>(a, tile, t, smem); break;            \
+      case 512: body<false, 512>(a, tile, t, smem); break;              \
+      case 256: body<false, 256>(a, tile, t, smem); break;              \
+      case 128: body<false, 128>(a, tile, t, smem); break;              \
+      default: body<false, 64>(a, tile, t, smem); break;                \
+    }                                                                   \
+  }
+
+__global__ void __launch_bounds__(kThreads, 3) gram_kernel(const StepParams a) {
+  extern __shared__ __align__(16) float smem[];
+  const Tile tile = a.tiles[blockIdx.x];
+  const Mat t = a.mats[tile.mat];
+  K2Q_BY_SHAPE(gram_body)
+}
+
 // S x S matrices of the iteration in shared memory: S8 rows, the padding zero; the pitch lets the 32 lanes of a
 // fragment read (8 rows, 4 neighbours each) meet all banks.
 __host__ __device__ constexpr int up8(int s) { return (s + 7) & ~7; }
 __host__ __device__ constexpr int pitch64(int s) { return ((s + 15) & ~15) + 4; }
 
-// For two commuting symmetric matrices: d = alpha I + beta y + gamma x y on the upper triangle and mirrored (alpha on the
-// first s entries of the diagonal).  A warp takes every eighth 8 x 8 tile.  x y is symmetric up to rounding in 64 bits,
-// so y's columns may be read as its rows.
-__device__ __forceinline__ void poly_step(double* d, const double* x, const double* y, int s, double alpha, double beta, double gamma) {
-  const int n8 = up8(s) >> 3, pitch = pitch64(s), lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
-  const int pairs = n8 * (n8 + 1) / 2;
-  constexpr int kWarps = kThreads / 32;
-  for (int e0 = threadIdx.x >> 5; e0 < pairs; e0 += 2 * kWarps) {      // two tiles at a time, two sums each: four chains
-    int it[2], jt[2];
-    double c[2][2][2] = {};
-    const double *xa[2], *yb[2];
+// A warp's 8 x 8 tiles of the upper triangle (it takes every WARPS-th), as element offsets in the shared matrices.  Eight
+// warps and two tiles each cover S = 32 and leave room for three matrices on an SM; beyond, 16 warps shorten the chain.
+template <int WARPS, int TILES>
+struct PolyTiles {
+  int n, pitch;
+  int xa[TILES], yb[TILES], ij[TILES], ji[TILES];
+  bool up0[TILES], up1[TILES];       // this lane's two entries lie on or above the diagonal
+  bool diag0[TILES], diag1[TILES];
+  __device__ __forceinline__ PolyTiles(int s) {
+    const int n8 = up8(s) >> 3, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3, pairs = n8 * (n8 + 1) / 2;
+    pitch = pitch64(s);
+    n = 0;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      int ti = 0, tj = e0 + w * kWarps < pairs ? e0 + w * kWarps : e0;   // past the end: the first once more, not stored
+    for (int k = 0; k < TILES; ++k) {
+      int ti = 0, tj = (threadIdx.x >> 5) + k * WARPS;
+      if (tj < pairs) n = k + 1;
+      else tj = 0;
       while (tj >= n8 - ti) { tj -= n8 - ti; ++ti; }
       tj += ti;
-      it[w] = 8 * ti + r;
-      jt[w] = 8 * tj + 2 * q;
-      xa[w] = x + (8 * ti + r) * pitch + q;
-      yb[w] = y + (8 * tj + r) * pitch + q;
+      const int i = 8 * ti + r, j = 8 * tj + 2 * q;
+      xa[k] = i * pitch + q;
+      yb[k] = (8 * tj + r) * pitch + q;
+      ij[k] = i * pitch + j;
+      ji[k] = j * pitch + i;
+      up0[k] = i <= j;
+      up1[k] = i <= j + 1;
+      diag0[k] = i == j && i < s;
+      diag1[k] = i == j + 1 && i < s;
     }
-#pragma unroll 2
-    for (int k = 0; k < 8 * n8; k += 8)
+  }
+};
+
+// For two commuting symmetric matrices: d = x y, or with FACTOR d = a I + b y + c x y; computed on the upper triangle and
+// mirrored.  x y is symmetric up to rounding in 64 bits, so y's columns may be read as its rows.
+template <bool FACTOR, int WARPS, int TILES>
+__device__ __forceinline__ void poly_step(double* d, const double* x, const double* y, const PolyTiles<WARPS, TILES>& t, int s8) {
+#pragma unroll
+  for (int k = 0; k < TILES; ++k) {
+    if (k >= t.n) break;
+    double c[2][2] = {};
+    const double *xa = x + t.xa[k], *yb = y + t.yb[k];
+#pragma unroll 4
+    for (int l = 0; l < s8; l += 8)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
-          asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};"
-              : "+d"(c[w][h][0]), "+d"(c[w][h][1])
-              : "d"(xa[w][k + 4 * h]), "d"(yb[w][k + 4 * h]));
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      if (e0 + w * kWarps >= pairs) break;
-      const int i = it[w], j = jt[w];
-      double c0 = gamma * (c[w][0][0] + c[w][1][0]), c1 = gamma * (c[w][0][1] + c[w][1][1]);
-      if (beta != 0.0) {
-        c0 += beta * y[i * pitch + j] + (i == j && i < s ? alpha : 0.0);
-        c1 += beta * y[i * pitch + j + 1] + (i == j + 1 && i < s ? alpha : 0.0);
-      }
-      if (i <= j) d[i * pitch + j] = d[j * pitch + i] = c0;      // one writer per entry, in diagonal tiles too
-      if (i <= j + 1) d[i * pitch + j + 1] = d[(j + 1) * pitch + i] = c1;
+        asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};"
+            : "+d"(c[h][0]), "+d"(c[h][1])
+            : "d"(xa[l + 4 * h]), "d"(yb[l + 4 * h]));
+    double c0 = c[0][0] + c[1][0], c1 = c[0][1] + c[1][1];
+    if (FACTOR) {
+      const double2 y2 = *reinterpret_cast<const double2*>(y + t.ij[k]);
+      c0 = kC * c0 + kB * y2.x + (t.diag0[k] ? kA : 0.0);
+      c1 = kC * c1 + kB * y2.y + (t.diag1[k] ? kA : 0.0);
     }
+    if (t.up0[k]) d[t.ij[k]] = d[t.ji[k]] = c0;                // one writer per entry, in diagonal tiles too
+    if (t.up1[k]) d[t.ij[k] + 1] = d[t.ji[k] + t.pitch] = c1;
   }
   __syncthreads();
 }
 
-__global__ void __launch_bounds__(kThreads) poly_kernel(const StepParams a) {
+template <int WARPS, int TILES>
+__global__ void __launch_bounds__(WARPS * 32) poly_kernel(const StepParams a) {
+  constexpr int kPolyThreads = WARPS * 32;
   extern __shared__ __align__(16) double sh[];
   __shared__ double inv;
   const Mat t = a.mats[blockIdx.x];
-  const int s4 = up4(t.s), nt = s4 >> 2, pairs = pairs_of(t.s), pitch = pitch64(t.s), n = up8(t.s) * pitch;
+  const int s4 = up4(t.s), s8 = up8(t.s), nt = s4 >> 2, pairs = pairs_of(t.s), pitch = pitch64(t.s), n = s8 * pitch;
   double *g = sh, *q = sh + n, *x = sh + 2 * n, *y = sh + 3 * n;
-  for (int e = threadIdx.x; e < n; e += kThreads) g[e] = 0.0;
+  const PolyTiles<WARPS, TILES> tiles(t.s);
+  for (int e = threadIdx.x; e < n; e += kPolyThreads) {
+    g[e] = 0.0;
+    if (a.steps == 0) x[e] = e / pitch == e % pitch ? 1.0 : 0.0;
+  }
   __syncthreads();
-  for (int e = threadIdx.x; e < pairs * 16; e += kThreads) {
+  for (int e = threadIdx.x; e < pairs * 16; e += kPolyThreads) {
     double v = 0.0;
     const float* part = a.ws + t.gram + e;
 #pragma unroll 8
@@ -393,32 +438,27 @@ __global__ void __launch_bounds__(kThreads) poly_kernel(const StepParams a) {
   }
   __syncthreads();
   const double f = inv;
-  for (int e = threadIdx.x; e < n; e += kThreads) {
-    g[e] *= f * f;
-    if (a.steps == 0) x[e] = e / pitch == e % pitch ? 1.0 : 0.0;
-  }
+  for (int e = threadIdx.x; e < n; e += kPolyThreads) g[e] *= f * f;
   __syncthreads();
   for (int it = 0; it < a.steps; ++it) {
     double* factor = it == 0 ? x : q;          // the first factor is the product so far
-    poly_step(factor, g, g, t.s, kA, kB, kC);
+    poly_step<true>(factor, g, g, tiles, s8);
     if (it > 0) {
-      poly_step(y, q, x, t.s, 0.0, 0.0, 1.0);
+      poly_step<false>(y, q, x, tiles, s8);
       double* o = x; x = y; y = o;
     }
     if (it + 1 < a.steps) {
       const double* f1 = it == 0 ? x : q;
-      poly_step(y, f1, g, t.s, 0.0, 0.0, 1.0);
-      poly_step(g, f1, y, t.s, 0.0, 0.0, 1.0);
+      poly_step<false>(y, f1, g, tiles, s8);
+      poly_step<false>(g, f1, y, tiles, s8);
     }
   }
-  for (int e = threadIdx.x; e < s4 * s4; e += kThreads) a.ws[t.poly + e] = static_cast<float>(x[e / s4 * pitch + e % s4] * f);
+  for (int e = threadIdx.x; e < s4 * s4; e += kPolyThreads) a.ws[t.poly + e] = static_cast<float>(x[e / s4 * pitch + e % s4] * f);
 }
 
-__global__ void __launch_bounds__(kThreads, 2) apply_kernel(const StepParams a) {
-  extern __shared__ __align__(16) float smem[];
-  const Tile tile = a.tiles[blockIdx.x];
-  const Mat t = a.mats[tile.mat];
-  const Place pl(t, a.aligned);
+template <bool TALL, int BLOCK>
+__device__ __forceinline__ void apply_body(const StepParams& a, const Tile& tile, const Mat& t, float* smem) {
+  const Place pl(t, a.aligned, TALL, BLOCK);
   const Share sh(pl);
   const float clip = clip_factor(a);
   const int64_t last = min(t.l, tile.first + a.piece);
@@ -561,6 +601,13 @@ __global__ void __launch_bounds__(kThreads, 2) apply_kernel(const StepParams a) 
   }
 }
 
+__global__ void __launch_bounds__(kThreads, 2) apply_kernel(const StepParams a) {
+  extern __shared__ __align__(16) float smem[];
+  const Tile tile = a.tiles[blockIdx.x];
+  const Mat t = a.mats[tile.mat];
+  K2Q_BY_SHAPE(apply_body)
+}
+
 // ---- host side ---------------------------------------------------------------------------------
 int make_plan(const char* name, const int64_t* rows, const int64_t* cols, int64_t count, k2q_matrices* out) {
   if (!rows || !cols || !out || count <= 0 || count > 0x7fffff) return fail(K2Q_EINVAL, "%s: bad arguments", name);
@@ -614,7 +661,8 @@ int run_steps(const char* name, const k2q_matrices* pl, const void* table, StepP
   if (int rc = check_cuda(cudaFuncSetAttribute(gram_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGramSmem),
                           "cudaFuncSetAttribute(gram)"))
     return rc;
-  if (int rc = check_cuda(cudaFuncSetAttribute(poly_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, poly_smem),
+  auto poly = pl->max_short <= 32 ? poly_kernel<8, 2> : poly_kernel<16, 3>;
+  if (int rc = check_cuda(cudaFuncSetAttribute(poly, cudaFuncAttributeMaxDynamicSharedMemorySize, poly_smem),
                           "cudaFuncSetAttribute(poly)"))
     return rc;
   if (int rc = check_cuda(cudaFuncSetAttribute(apply_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, apply_smem),
@@ -622,7 +670,7 @@ int run_steps(const char* name, const k2q_matrices* pl, const void* table, StepP
     return rc;
   const unsigned tiles = static_cast<unsigned>(pl->tiles);
   gram_kernel<<<tiles, kThreads, kGramSmem, s>>>(a);
-  poly_kernel<<<static_cast<unsigned>(pl->count), kThreads, poly_smem, s>>>(a);
+  poly<<<static_cast<unsigned>(pl->count), pl->max_short <= 32 ? 256 : 512, poly_smem, s>>>(a);
   apply_kernel<<<tiles, kThreads, apply_smem, s>>>(a);
   return check_cuda(cudaGetLastError(), name);
 }
