@@ -42,6 +42,13 @@ __device__ __forceinline__ void load8f(const float* p, float* v) {
 __device__ __forceinline__ uint4 load_row16(const __nv_bfloat16* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }
 __device__ __forceinline__ uint4 load_vec16(const __nv_bfloat16* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
+// maximum that keeps a NaN: a row with one gets a NaN scale, not small codes
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // Sum / maximum over the CTA, the same value in every thread, in a fixed order.  One barrier: successive
 // calls of a kernel alternate between two slots, so a slot is written again only behind the barrier of
 // the call in between, which every reader of the slot has passed.
@@ -50,12 +57,12 @@ __device__ __forceinline__ float cta_reduce(float v, float* slot, int warps) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float other = __shfl_xor_sync(0xffffffffu, v, o);
-    v = MAX ? fmaxf(v, other) : v + other;
+    v = MAX ? max_nan(v, other) : v + other;
   }
   if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
   __syncthreads();
   float t = slot[0];
-  for (int w = 1; w < warps; ++w) t = MAX ? fmaxf(t, slot[w]) : t + slot[w];
+  for (int w = 1; w < warps; ++w) t = MAX ? max_nan(t, slot[w]) : t + slot[w];
   return t;
 }
 
@@ -76,24 +83,9 @@ struct ResParams {
   const __nv_bfloat16* dh; int64_t lddh;        // or NULL
   __nv_bfloat16* dx; int64_t lddx;              // or NULL
   __nv_bfloat16* dy; int64_t lddy;              // or NULL
-  float* part; int chunks;                      // [B, chunks, 3, K] partial sums D, S, H, or NULL
+  float* part;                                  // [B, chunks, 3, K] partial sums D, S, H, or NULL
+  int chunks;                                   // CTAs per sample
 };
-
-// stream of 8 consecutive elements; rounded product and rounded sum, as the two fp32 operations it is
-__device__ __forceinline__ uint4 residual8(const ResParams& p, int64_t row, int64_t b, int k0) {
-  float x[8], y[8];
-  unpack8(load_row16(p.x + row * p.ldx + k0), x);
-  unpack8(load_row16(p.y + row * p.ldy + k0), y);
-  if (p.gate != nullptr) {
-    float g[8];
-    unpack8(load_vec16(p.gate + b * p.K + k0), g);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = __fmul_rn(g[e], y[e]);
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(x[e], y[e]);
-  return pack8(x);
-}
 
 // h of 8 consecutive elements from the kept stream
 __device__ __forceinline__ void norm_mod8(const ResParams& p, int64_t b, int k0, float rstd, float* v) {
@@ -116,194 +108,387 @@ __device__ __forceinline__ void norm_mod8(const ResParams& p, int64_t b, int k0,
 }
 
 // ---- sampling: rotated int8 codes -------------------------------------------------------------
-// One CTA per row, four neighbouring lanes per 128-block.  Lane q of the four owns the 8-element chunks
-// q, q + 4, q + 8, q + 12 of the block: a warp's 16-byte accesses then cover whole 64-byte pieces (32-byte
-// pieces of the codes), and no staging through shared memory is needed.  Of the rotation's seven
-// butterfly stages, h = 1, 2, 4 and 32, 64 lie inside a thread, h = 8 and 16 between lanes.
-__device__ __forceinline__ void fwht128_chunks(float (&v)[32], int q) {
+// A CTA works through consecutive rows of one sample.  Its vectors are combined once, in shared memory:
+//   f = (1 + w)(1 + sc) c,  s = sh c   (fp32; c the rotation's normalisation, which commutes with it)  and the gate,
+// so that a row costs one packed bf16 multiply-add per two elements for the stream and one packed fp32 one for h.  Four
+// neighbouring lanes hold a 128-block.  Lane q of the four owns the 8-element chunks q, q + 4, q + 8, q + 12 of the
+// block: a warp's 16-byte accesses then cover whole 64-byte pieces (32-byte pieces of the codes), and nothing has to be
+// staged through shared memory.  Of the rotation's seven butterfly stages, h = 1, 2, 4 and 32, 64 lie inside a thread,
+// h = 8 and 16 between lanes.  The next row is requested before the current one is worked on.
+__device__ __forceinline__ void fwht128_chunks(uint64_t (&p)[16], int q) {
+  const uint64_t neg2 = pack_f32x2(-1.0f, -1.0f);
 #pragma unroll
-  for (int h = 1; h < 8; h <<= 1) {
+  for (int i = 0; i < 16; ++i) {
+    float a, b;
+    unpack_f32x2(p[i], a, b);
+    p[i] = pack_f32x2(__fadd_rn(a, b), __fsub_rn(a, b));
+  }
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+  for (int h = 1; h < 4; h <<= 1) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
       if ((i & h) == 0) {
-        const float a = v[i], b = v[i + h];
-        v[i] = __fadd_rn(a, b);
-        v[i + h] = __fsub_rn(a, b);
+        const uint64_t a = p[i], b = p[i + h];
+        p[i] = add_f32x2(a, b);
+        p[i + h] = fma_f32x2(b, neg2, a);
       }
     }
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const float sgn = ((q >> j) & 1) ? -1.0f : 1.0f;     // lower lane a + b, upper lane a - b
+    const uint64_t sgn2 = pack_f32x2(sgn, sgn);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float o = __shfl_xor_sync(0xffffffffu, v[i], 1 << j);
-      v[i] = __fmaf_rn(v[i], sgn, o);
+    for (int i = 0; i < 16; ++i) {
+      float a, b;
+      unpack_f32x2(p[i], a, b);
+      const float oa = __shfl_xor_sync(0xffffffffu, a, 1 << j), ob = __shfl_xor_sync(0xffffffffu, b, 1 << j);
+      p[i] = fma_f32x2(p[i], sgn2, pack_f32x2(oa, ob));
     }
   }
 #pragma unroll
-  for (int h = 8; h < 32; h <<= 1) {
+  for (int h = 4; h < 16; h <<= 1) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < 16; ++i) {
       if ((i & h) == 0) {
-        const float a = v[i], b = v[i + h];
-        v[i] = __fadd_rn(a, b);
-        v[i + h] = __fsub_rn(a, b);
+        const uint64_t a = p[i], b = p[i + h];
+        p[i] = add_f32x2(a, b);
+        p[i + h] = fma_f32x2(b, neg2, a);
       }
     }
   }
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] *= kHadNorm;
 }
 
+// bf16 pairs, each half rounded once (the product of two bf16 values is not rounded on its own)
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t widen2(uint32_t w) { return pack_f32x2(w << 16, w & 0xFFFF0000u); }
+
+struct RowChunks { uint4 x[4], y[4]; };
+
+// rows [r0, r1) of sample b that CTA blockIdx.x = b * chunks + chunk works on
+__device__ __forceinline__ void cta_rows(const ResParams& p, int64_t& b, int64_t& r0, int64_t& r1) {
+  b = blockIdx.x / p.chunks;
+  const int chunk = blockIdx.x - static_cast<int>(b) * p.chunks;
+  r0 = b * p.rows_per_batch + p.rows_per_batch * chunk / p.chunks;
+  r1 = b * p.rows_per_batch + p.rows_per_batch * (chunk + 1) / p.chunks;
+}
+
+template <bool GATE, bool SHIFT>
 __global__ void __launch_bounds__(512) residual_quant_kernel(const ResParams p) {
+  extern __shared__ __align__(16) float vec[];                 // f [K] | s [K] (SHIFT) | gate [K] bf16 (GATE)
   __shared__ float red[2][kMaxWarps];
+  float* s_s = vec + p.K;
+  const uint32_t* s_g = reinterpret_cast<const uint32_t*>(vec + (SHIFT ? 2 : 1) * p.K);
   const int warps = blockDim.x >> 5;
   const int q = threadIdx.x & 3;
-  const int blk = threadIdx.x >> 2;                       // 128-block of the row
+  const int blk = threadIdx.x >> 2;                            // 128-block of the row
   const bool own = blk < (p.K >> 7);
-  for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
-    const int64_t b = row / p.rows_per_batch;
-    float v[32];
-    float ss = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int k0 = blk * 128 + (q + 4 * j) * 8;
-      if (own) {
-        const uint4 s = residual8(p, row, b, k0);
-        *reinterpret_cast<uint4*>(p.stream + row * p.lds + k0) = s;
-        unpack8(s, v + 8 * j);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[8 * j + e] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 32; ++i) ss = fmaf(v[i], v[i], ss);
-    const float rstd = rsqrtf(cta_reduce<false>(ss, red[0], warps) / static_cast<float>(p.K) + p.eps);
+  const int k00 = blk * 128 + q * 8;                           // first chunk; the others 32 elements apart
+  int64_t b, r0, r1;
+  cta_rows(p, b, r0, r1);
+  pdl_wait();
+
+  auto fetch = [&](int64_t row, RowChunks& c) {
     if (own) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) norm_mod8(p, b, blk * 128 + (q + 4 * j) * 8, rstd, v + 8 * j);
+      for (int j = 0; j < 4; ++j) {
+        c.x[j] = load_row16(p.x + row * p.ldx + k00 + 32 * j);
+        c.y[j] = load_row16(p.y + row * p.ldy + k00 + 32 * j);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c.x[j] = c.y[j] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  RowChunks next;
+  fetch(r0, next);
+  for (int c = threadIdx.x; c < (p.K >> 3); c += blockDim.x) {
+    const int k = 8 * c;
+    float f[8];
+    load8f(p.normw + k, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (1.0f + f[e]) * kHadNorm;
+    if (p.mscale != nullptr) {
+      float s[8];
+      unpack8(load_vec16(p.mscale + b * p.K + k), s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= 1.0f + s[e];
+    }
+    *reinterpret_cast<float4*>(vec + k) = make_float4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<float4*>(vec + k + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    if (SHIFT) {
+      float s[8];
+      unpack8(load_vec16(p.mshift + b * p.K + k), s);
+      *reinterpret_cast<float4*>(s_s + k) = make_float4(s[0] * kHadNorm, s[1] * kHadNorm, s[2] * kHadNorm, s[3] * kHadNorm);
+      *reinterpret_cast<float4*>(s_s + k + 4) = make_float4(s[4] * kHadNorm, s[5] * kHadNorm, s[6] * kHadNorm, s[7] * kHadNorm);
+    }
+    if (GATE) *reinterpret_cast<uint4*>(vec + (SHIFT ? 2 : 1) * p.K + (k >> 1)) = load_vec16(p.gate + b * p.K + k);
+  }
+  __syncthreads();
+
+  const float inv_k = 1.0f / static_cast<float>(p.K);
+  for (int64_t row = r0; row < r1; ++row) {
+    uint64_t v[16];
+    uint64_t ss2[2] = {0ull, 0ull};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint4 s = next.x[j];
+      const uint4 y = next.y[j];
+      uint4 g = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u);   // one
+      if (GATE && own) g = *reinterpret_cast<const uint4*>(s_g + ((k00 + 32 * j) >> 1));
+      s.x = fma_bf16x2(g.x, y.x, s.x); s.y = fma_bf16x2(g.y, y.y, s.y);
+      s.z = fma_bf16x2(g.z, y.z, s.z); s.w = fma_bf16x2(g.w, y.w, s.w);
+      if (own) *reinterpret_cast<uint4*>(p.stream + row * p.lds + k00 + 32 * j) = s;
+      v[4 * j] = widen2(s.x); v[4 * j + 1] = widen2(s.y); v[4 * j + 2] = widen2(s.z); v[4 * j + 3] = widen2(s.w);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ss2[e & 1] = fma_f32x2(v[4 * j + e], v[4 * j + e], ss2[e & 1]);
+    }
+    if (row + 1 < r1) fetch(row + 1, next);
+    float a0, a1, a2, a3;
+    unpack_f32x2(ss2[0], a0, a1);
+    unpack_f32x2(ss2[1], a2, a3);
+    const float rstd = rsqrtf(cta_reduce<false>((a0 + a1) + (a2 + a3), red[0], warps) * inv_k + p.eps);
+    const uint64_t rstd2 = pack_f32x2(rstd, rstd);
+    if (own) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const ulonglong2 f0 = *reinterpret_cast<const ulonglong2*>(vec + k00 + 32 * j), f1 = *reinterpret_cast<const ulonglong2*>(vec + k00 + 32 * j + 4);
+        const uint64_t f[4] = {f0.x, f0.y, f1.x, f1.y};
+        if (SHIFT) {
+          const ulonglong2 s0 = *reinterpret_cast<const ulonglong2*>(s_s + k00 + 32 * j), s1 = *reinterpret_cast<const ulonglong2*>(s_s + k00 + 32 * j + 4);
+          const uint64_t s[4] = {s0.x, s0.y, s1.x, s1.y};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * j + e] = fma_f32x2(mul_f32x2(v[4 * j + e], rstd2), f[e], s[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * j + e] = mul_f32x2(mul_f32x2(v[4 * j + e], rstd2), f[e]);
+        }
+      }
     }
     fwht128_chunks(v, q);
-    float amax = 0.f;
+    float m0 = 0.f, m1 = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(v[i]));
-    amax = cta_reduce<true>(amax, red[1], warps);
-    const float s = __fdiv_rn(fmaxf(amax, 1e-8f), 127.0f);
+    for (int i = 0; i < 16; ++i) {
+      float a, c;
+      unpack_f32x2(v[i], a, c);
+      m0 = max_nan(m0, fabsf(a));
+      m1 = max_nan(m1, fabsf(c));
+    }
+    const float s = __fdiv_rn(max_nan(cta_reduce<true>(max_nan(m0, m1), red[1], warps), 1e-8f), 127.0f);
     const float inv = __frcp_rn(s);
+    // v / s + 1.5 * 2^23 carries the rounded code in its low byte
+    const uint64_t inv2 = pack_f32x2(inv, inv), magic2 = pack_f32x2(kRoundMagic, kRoundMagic);
     uint32_t words[8];
-    quant_row32_i8(v, s, inv, words);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      float c0, c1, c2, c3;
+      unpack_f32x2(fma_f32x2(v[2 * w], inv2, magic2), c0, c1);
+      unpack_f32x2(fma_f32x2(v[2 * w + 1], inv2, magic2), c2, c3);
+      words[w] = prmt_b(prmt_b(__float_as_uint(c0), __float_as_uint(c1), 0x0040u), prmt_b(__float_as_uint(c2), __float_as_uint(c3), 0x0040u), 0x5410u);
+    }
     if (own) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<uint2*>(p.xq + row * p.K + blk * 128 + (q + 4 * j) * 8) = make_uint2(words[2 * j], words[2 * j + 1]);
+        *reinterpret_cast<uint2*>(p.xq + row * p.K + k00 + 32 * j) = make_uint2(words[2 * j], words[2 * j + 1]);
     }
     if (threadIdx.x == 0) p.sx[row] = s;
   }
 }
 
 // ---- training: dense output and its backward ------------------------------------------------------
+// Both: a CTA works through consecutive rows of one sample, a thread owns the same columns in all of them; the next row
+// is requested before the current one is worked on, and the sample's vectors stay in registers, combined.
 template <int VPT>
 __global__ void __launch_bounds__(512) residual_fwd_kernel(const ResParams p) {
   __shared__ float red[2][kMaxWarps];
   const int warps = blockDim.x >> 5, nvec = p.K >> 3;
+  int64_t b, r0, r1;
+  cta_rows(p, b, r0, r1);
+  pdl_wait();
+  uint4 nx[VPT], ny[VPT];
+  auto fetch = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      if (c < nvec) {
+        nx[i] = load_row16(p.x + row * p.ldx + 8 * c);
+        ny[i] = load_row16(p.y + row * p.ldy + 8 * c);
+      }
+    }
+  };
+  fetch(r0);
   int it = 0;
-  for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x, it ^= 1) {
-    const int64_t b = row / p.rows_per_batch;
-    float v[VPT][8];
+  for (int64_t row = r0; row < r1; ++row, it ^= 1) {
+    uint4 sv[VPT];
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
       if (c < nvec) {
-        const uint4 s = residual8(p, row, b, 8 * c);
+        uint4 g = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u);   // one
+        if (p.gate != nullptr) g = load_vec16(p.gate + b * p.K + 8 * c);
+        uint4 s = nx[i];
+        s.x = fma_bf16x2(g.x, ny[i].x, s.x); s.y = fma_bf16x2(g.y, ny[i].y, s.y);
+        s.z = fma_bf16x2(g.z, ny[i].z, s.z); s.w = fma_bf16x2(g.w, ny[i].w, s.w);
         reinterpret_cast<uint4*>(p.stream + row * p.lds)[c] = s;
-        unpack8(s, v[i]);
+        sv[i] = s;
+        float v[8];
+        unpack8(s, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(v[i][e], v[i][e], ss);
+        for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
       }
     }
+    if (row + 1 < r1) fetch(row + 1);
     const float rstd = rsqrtf(cta_reduce<false>(ss, red[it], warps) / static_cast<float>(p.K) + p.eps);
     if (threadIdx.x == 0) p.rstd[row] = rstd;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
       if (c < nvec) {
-        norm_mod8(p, b, 8 * c, rstd, v[i]);
-        reinterpret_cast<uint4*>(p.h + row * p.ldh)[c] = pack8(v[i]);
+        float v[8];
+        unpack8(sv[i], v);
+        norm_mod8(p, b, 8 * c, rstd, v);
+        reinterpret_cast<uint4*>(p.h + row * p.ldh)[c] = pack8(v);
       }
     }
   }
 }
 
-// A CTA works through consecutive rows of ONE sample and a thread owns the same columns in all of them, so
-// the sums over rows stay in registers; each CTA leaves its partial sums in its own slice of the workspace.
+// SUMS: each CTA adds up its rows' terms of D, S and H, in registers (one vector per thread) or in its shared memory
+// (several: 96 sums would not fit beside the rows), and leaves them in its own slice of the workspace.
+// Up to two vectors per thread the next row is requested before the current one is worked on, and the sample's
+// (1 + w)(1 + sc) stays in registers; beyond, registers hold one row and the vectors are read again (L2).
 template <int VPT, bool SUMS>
 __global__ void __launch_bounds__(512) residual_bwd_kernel(const ResParams p) {
+  constexpr bool PRE = VPT <= 2, SHARED = SUMS && VPT > 1;
+  constexpr int Y = SUMS ? VPT : 1, W = PRE ? VPT : 1, A = SUMS && !SHARED ? 1 : 0;
+  extern __shared__ __align__(16) float sums[];                // SHARED: D [K], S [K], H [K]
   __shared__ float red[2][kMaxWarps];
   const int warps = blockDim.x >> 5, nvec = p.K >> 3;
-  const int64_t b = blockIdx.x / p.chunks;
-  const int chunk = blockIdx.x - static_cast<int>(b) * p.chunks;
-  const int64_t r0 = b * p.rows_per_batch + p.rows_per_batch * chunk / p.chunks;
-  const int64_t r1 = b * p.rows_per_batch + p.rows_per_batch * (chunk + 1) / p.chunks;
-  float aD[SUMS ? VPT : 1][8] = {}, aS[SUMS ? VPT : 1][8] = {}, aH[SUMS ? VPT : 1][8] = {};
-  int it = 0;
-  for (int64_t row = r0; row < r1; ++row, it ^= 1) {
-    float n[VPT][8], g[VPT][8];
-    float dot = 0.f, rstd = 0.f;
-    if (p.dh != nullptr) {
-      rstd = p.rstd[row];
+  int64_t b, r0, r1;
+  cta_rows(p, b, r0, r1);
+  pdl_wait();
+  const bool has_h = p.dh != nullptr, has_s = p.dstream != nullptr, sum_d = SUMS && p.y != nullptr;
+  float acc[A ? 3 : 1][8] = {};
+  uint4 n_ds[VPT], n_dh[VPT], n_st[VPT], n_y[Y];
+  float n_rstd = 0.f;
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int c = threadIdx.x + i * blockDim.x;
-        if (c < nvec) {
-          float w[8];
-          unpack8(load_vec16(p.dh + row * p.lddh + 8 * c), g[i]);
-          unpack8(load_vec16(p.stream + row * p.lds + 8 * c), n[i]);
-          load8f(p.normw + 8 * c, w);
+  for (int i = 0; i < VPT; ++i) n_ds[i] = n_dh[i] = n_st[i] = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] += 1.0f;
-          if (p.mscale != nullptr) {
-            float s[8];
-            unpack8(load_vec16(p.mscale + b * p.K + 8 * c), s);
+  for (int i = 0; i < Y; ++i) n_y[i] = make_uint4(0u, 0u, 0u, 0u);
+  auto fetch = [&](int64_t row) {
+    if (has_h) n_rstd = __ldg(p.rstd + row);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] *= 1.0f + s[e];
-          }
+    for (int i = 0; i < VPT; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      if (c < nvec) {
+        if (has_h) {
+          n_dh[i] = __ldcs(reinterpret_cast<const uint4*>(p.dh + row * p.lddh) + c);
+          n_st[i] = __ldcs(reinterpret_cast<const uint4*>(p.stream + row * p.lds) + c);
+        }
+        if (has_s) n_ds[i] = __ldcs(reinterpret_cast<const uint4*>(p.dstream + row * p.ldds) + c);
+        if (sum_d) n_y[SUMS ? i : 0] = __ldcs(reinterpret_cast<const uint4*>(p.y + row * p.ldy) + c);
+      }
+    }
+  };
+  auto weights = [&](int c, float* w) {
+    load8f(p.normw + 8 * c, w);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            n[i][e] *= rstd;
-            if (SUMS) {
-              aS[i][e] = fmaf(g[i][e], n[i][e], aS[i][e]);
-              aH[i][e] += g[i][e];
-            }
-            g[i][e] *= w[e];
-            dot = fmaf(g[i][e], n[i][e], dot);
-          }
+    for (int e = 0; e < 8; ++e) w[e] += 1.0f;
+    if (p.mscale != nullptr) {
+      float s[8];
+      unpack8(load_vec16(p.mscale + b * p.K + 8 * c), s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] *= 1.0f + s[e];
+    }
+  };
+  fetch(r0);                                                   // chunks <= rows_per_batch: there is a row
+  float w_keep[W][8];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    if (c < nvec) {
+      if (PRE) weights(c, w_keep[PRE ? i : 0]);
+      if (SHARED) {
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          *reinterpret_cast<float4*>(sums + j * p.K + 8 * c) = make_float4(0.f, 0.f, 0.f, 0.f);
+          *reinterpret_cast<float4*>(sums + j * p.K + 8 * c + 4) = make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
-      dot = cta_reduce<false>(dot, red[it], warps) / static_cast<float>(p.K);
     }
+  }
+  // adds v[e] * u[e] (or v[e] with u NULL) to a sum of this thread's columns 8c ..
+  auto add = [&](int j, int c, const float* v, const float* u) {
+    if (A) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[A ? j : 0][e] = u != nullptr ? fmaf(v[e], u[e], acc[A ? j : 0][e]) : acc[A ? j : 0][e] + v[e];
+    } else {
+#pragma unroll
+      for (int h = 0; h < 8; h += 4) {
+        float4* at = reinterpret_cast<float4*>(sums + j * p.K + 8 * c + h);
+        float4 s = *at;
+        s.x = u != nullptr ? fmaf(v[h], u[h], s.x) : s.x + v[h];
+        s.y = u != nullptr ? fmaf(v[h + 1], u[h + 1], s.y) : s.y + v[h + 1];
+        s.z = u != nullptr ? fmaf(v[h + 2], u[h + 2], s.z) : s.z + v[h + 2];
+        s.w = u != nullptr ? fmaf(v[h + 3], u[h + 3], s.w) : s.w + v[h + 3];
+        *at = s;
+      }
+    }
+  };
+  const float inv_k = 1.0f / static_cast<float>(p.K);
+  int it = 0;
+  for (int64_t row = r0; row < r1; ++row, it ^= 1) {
+    if (!PRE && row > r0) fetch(row);
+    uint4 c_ds[VPT], c_dh[VPT], c_st[VPT], c_y[Y];
+    const float rstd = n_rstd;
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      c_ds[i] = n_ds[i]; c_dh[i] = n_dh[i]; c_st[i] = n_st[i];
+      if (SUMS) c_y[SUMS ? i : 0] = n_y[SUMS ? i : 0];
+      if (c < nvec) {
+        float g[8], n[8], w[8];
+        unpack8(c_dh[i], g);
+        unpack8(c_st[i], n);
+        if (!PRE) weights(c, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) n[e] *= rstd;
+        if (SUMS) {
+          add(1, c, g, n);
+          add(2, c, g, nullptr);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot = fmaf(g[e] * (PRE ? w_keep[PRE ? i : 0][e] : w[e]), n[e], dot);
+      }
+    }
+    if (PRE && row + 1 < r1) fetch(row + 1);
+    if (has_h) dot = cta_reduce<false>(dot, red[it], warps) * inv_k;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
       if (c < nvec) {
         float d[8];
-        if (p.dstream != nullptr) unpack8(load_vec16(p.dstream + row * p.ldds + 8 * c), d);
-        else {
+        unpack8(c_ds[i], d);
+        if (has_h) {
+          float g[8], n[8], w[8];
+          unpack8(c_dh[i], g);
+          unpack8(c_st[i], n);
+          if (!PRE) weights(c, w);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) d[e] = 0.f;
+          for (int e = 0; e < 8; ++e)
+            d[e] += rstd * (g[e] * (PRE ? w_keep[PRE ? i : 0][e] : w[e]) - n[e] * rstd * dot);
         }
-        if (p.dh != nullptr) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d[e] += rstd * (g[i][e] - n[i][e] * dot);
-        }
-        if (p.dx != nullptr) reinterpret_cast<uint4*>(p.dx + row * p.lddx)[c] = pack8(d);
-        if (SUMS && p.gate != nullptr && p.y != nullptr) {
+        if (p.dx != nullptr) __stcs(reinterpret_cast<uint4*>(p.dx + row * p.lddx) + c, pack8(d));
+        if (sum_d) {
           float y[8];
-          unpack8(load_vec16(p.y + row * p.ldy + 8 * c), y);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) aD[i][e] = fmaf(d[e], y[e], aD[i][e]);
+          unpack8(c_y[SUMS ? i : 0], y);
+          add(0, c, d, y);
         }
         if (p.dy != nullptr) {
           if (p.gate != nullptr) {
@@ -312,7 +497,7 @@ __global__ void __launch_bounds__(512) residual_bwd_kernel(const ResParams p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) d[e] *= gt[e];
           }
-          reinterpret_cast<uint4*>(p.dy + row * p.lddy)[c] = pack8(d);
+          __stcs(reinterpret_cast<uint4*>(p.dy + row * p.lddy) + c, pack8(d));
         }
       }
     }
@@ -324,11 +509,12 @@ __global__ void __launch_bounds__(512) residual_bwd_kernel(const ResParams p) {
       const int c = threadIdx.x + i * blockDim.x;
       if (c < nvec) {
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-          *reinterpret_cast<float4*>(part + 8 * c + e) = make_float4(aD[i][e], aD[i][e + 1], aD[i][e + 2], aD[i][e + 3]);
-          *reinterpret_cast<float4*>(part + p.K + 8 * c + e) = make_float4(aS[i][e], aS[i][e + 1], aS[i][e + 2], aS[i][e + 3]);
-          *reinterpret_cast<float4*>(part + 2 * p.K + 8 * c + e) = make_float4(aH[i][e], aH[i][e + 1], aH[i][e + 2], aH[i][e + 3]);
-        }
+        for (int j = 0; j < 3; ++j)
+#pragma unroll
+          for (int h = 0; h < 8; h += 4)
+            *reinterpret_cast<float4*>(part + j * p.K + 8 * c + h) =
+                SHARED ? *reinterpret_cast<const float4*>(sums + j * p.K + 8 * c + h)
+                       : make_float4(acc[A ? j : 0][h], acc[A ? j : 0][h + 1], acc[A ? j : 0][h + 2], acc[A ? j : 0][h + 3]);
       }
     }
   }
@@ -392,11 +578,15 @@ int check_common(const char* name, const ResParams& p, int64_t K, int unit) {
   return K2Q_OK;
 }
 
-int grid_rows(int64_t rows, int ctas_per_sm) {
+// CTAs per sample: enough for `ctas_per_sm` on every SM over all samples, at most one per row
+int chunks_for(int64_t B, int64_t rows_per_batch, int ctas_per_sm) {
   const int sms = sm_count() > 0 ? sm_count() : 148;
-  const int64_t most = static_cast<int64_t>(sms) * ctas_per_sm;
-  return static_cast<int>(rows < most ? rows : most);
+  int64_t c = (static_cast<int64_t>(sms) * ctas_per_sm + B - 1) / B;
+  if (c > rows_per_batch) c = rows_per_batch;
+  return static_cast<int>(c < 1 ? 1 : c);
 }
+// CTAs of the dense kernels that share an SM: about 768 threads
+int dense_ctas(int threads) { return threads >= 512 ? 1 : 768 / threads; }
 
 // threads per CTA and 16-byte vectors per thread of the dense kernels
 void dense_shape(int64_t K, int* threads, int* vpt) {
@@ -431,8 +621,23 @@ int k2q_residual_norm_quant(const void* x_bf16, int64_t ldx, const void* y_bf16,
   if (bad_rows(p.x, ldx, K) || bad_rows(p.y, ldy, K) || bad_rows(p.stream, lds, K) || off16(xq))
     return fail(K2Q_EINVAL, "%s: rows must be 16-byte aligned with a leading dimension >= K", name);
   const int threads = (static_cast<int>(K / 32) + 31) / 32 * 32;
-  residual_quant_kernel<<<grid_rows(M, 32), threads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  return check_cuda(cudaGetLastError(), "residual_quant launch");
+  const int64_t B = M / rows_per_batch;
+  // registers let about 640 threads share an SM, the vectors in shared memory must fit as often
+  const int vec_bytes = static_cast<int>(K) * (4 + (p.mshift ? 4 : 0) + (p.gate ? 2 : 0));
+  int ctas = threads >= 640 ? 1 : 640 / threads;
+  if (ctas > 220 * 1024 / (vec_bytes + 1024)) ctas = 220 * 1024 / (vec_bytes + 1024);
+  if (ctas > 16) ctas = 16;
+  p.chunks = chunks_for(B, rows_per_batch, ctas < 1 ? 1 : ctas);
+  if (B * p.chunks > 0x7fffffffLL) return fail(K2Q_EINVAL, "%s: too many samples (%lld)", name, (long long)B);
+  auto kern = p.gate ? (p.mshift ? residual_quant_kernel<true, true> : residual_quant_kernel<true, false>)
+                     : (p.mshift ? residual_quant_kernel<false, true> : residual_quant_kernel<false, false>);
+  if (vec_bytes > 48 * 1024) {
+    if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, vec_bytes),
+                            "cudaFuncSetAttribute(residual_quant)"))
+      return rc;
+  }
+  return launch_overlapped(kern, static_cast<unsigned>(B * p.chunks), static_cast<unsigned>(threads), static_cast<size_t>(vec_bytes),
+                           static_cast<cudaStream_t>(stream), 1, "residual_quant launch", p);
 }
 
 int k2q_residual_norm_fwd(const void* x_bf16, int64_t ldx, const void* y_bf16, int64_t ldy, const void* gate_bf16,
@@ -456,28 +661,24 @@ int k2q_residual_norm_fwd(const void* x_bf16, int64_t ldx, const void* y_bf16, i
     return fail(K2Q_EINVAL, "%s: rows must be 16-byte aligned with a leading dimension >= K", name);
   int threads, vpt;
   dense_shape(K, &threads, &vpt);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int grid = grid_rows(M, 32);
-  switch (vpt) {
-    case 1: residual_fwd_kernel<1><<<grid, threads, 0, s>>>(p); break;
-    case 2: residual_fwd_kernel<2><<<grid, threads, 0, s>>>(p); break;
-    case 3: residual_fwd_kernel<3><<<grid, threads, 0, s>>>(p); break;
-    default: residual_fwd_kernel<4><<<grid, threads, 0, s>>>(p); break;
-  }
-  return check_cuda(cudaGetLastError(), "residual_fwd launch");
+  const int64_t B = M / rows_per_batch;
+  p.chunks = chunks_for(B, rows_per_batch, dense_ctas(threads));
+  if (B * p.chunks > 0x7fffffffLL) return fail(K2Q_EINVAL, "%s: too many samples (%lld)", name, (long long)B);
+  auto kern = vpt == 1 ? residual_fwd_kernel<1> : vpt == 2 ? residual_fwd_kernel<2> : vpt == 3 ? residual_fwd_kernel<3> : residual_fwd_kernel<4>;
+  return launch_overlapped(kern, static_cast<unsigned>(B * p.chunks), static_cast<unsigned>(threads), 0, static_cast<cudaStream_t>(stream), 1,
+                           "residual_fwd launch", p);
 }
 
-static int bwd_chunks(int64_t B, int64_t rows_per_batch) {
-  const int sms = sm_count() > 0 ? sm_count() : 148;
-  int64_t c = (2LL * sms + B - 1) / B;
-  if (c > rows_per_batch) c = rows_per_batch;
-  return static_cast<int>(c < 1 ? 1 : c);
+static int bwd_chunks(int64_t B, int64_t rows_per_batch, int64_t K) {
+  int threads, vpt;
+  dense_shape(K, &threads, &vpt);
+  return chunks_for(B, rows_per_batch, dense_ctas(threads));
 }
 
 int64_t k2q_residual_norm_bwd_workspace_bytes(int64_t rows_per_batch, int64_t M, int64_t K) {
   if (rows_per_batch <= 0 || M <= 0 || K <= 0) return 0;
   const int64_t B = M / rows_per_batch;
-  return B * bwd_chunks(B, rows_per_batch) * 3 * K * static_cast<int64_t>(sizeof(float));
+  return B * bwd_chunks(B, rows_per_batch, K) * 3 * K * static_cast<int64_t>(sizeof(float));
 }
 
 int k2q_residual_norm_bwd(const void* dstream_bf16, int64_t ldds, const void* dh_bf16, int64_t lddh,
@@ -508,7 +709,7 @@ int k2q_residual_norm_bwd(const void* dstream_bf16, int64_t ldds, const void* dh
   if (dgate_bf16 && (!p.gate || !p.y)) return fail(K2Q_EINVAL, "%s: the gate's gradient needs gate and y", name);
   const int64_t B = M / rows_per_batch;
   const bool sums = dgate_bf16 || dmod_scale_bf16 || dmod_shift_bf16 || dnorm;
-  p.chunks = bwd_chunks(B, rows_per_batch);
+  p.chunks = bwd_chunks(B, rows_per_batch, K);
   if (!dgate_bf16) p.y = nullptr;
   if (sums) {
     if (!ws || off16(ws) || ws_bytes < k2q_residual_norm_bwd_workspace_bytes(rows_per_batch, M, K))
@@ -520,17 +721,25 @@ int k2q_residual_norm_bwd(const void* dstream_bf16, int64_t ldds, const void* dh
   dense_shape(K, &threads, &vpt);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(B * p.chunks);
+  void (*kern)(ResParams) = nullptr;
   switch (vpt * 2 + (sums ? 1 : 0)) {
-    case 2: residual_bwd_kernel<1, false><<<grid, threads, 0, s>>>(p); break;
-    case 3: residual_bwd_kernel<1, true><<<grid, threads, 0, s>>>(p); break;
-    case 4: residual_bwd_kernel<2, false><<<grid, threads, 0, s>>>(p); break;
-    case 5: residual_bwd_kernel<2, true><<<grid, threads, 0, s>>>(p); break;
-    case 6: residual_bwd_kernel<3, false><<<grid, threads, 0, s>>>(p); break;
-    case 7: residual_bwd_kernel<3, true><<<grid, threads, 0, s>>>(p); break;
-    case 8: residual_bwd_kernel<4, false><<<grid, threads, 0, s>>>(p); break;
-    default: residual_bwd_kernel<4, true><<<grid, threads, 0, s>>>(p); break;
+    case 2: kern = residual_bwd_kernel<1, false>; break;
+    case 3: kern = residual_bwd_kernel<1, true>; break;
+    case 4: kern = residual_bwd_kernel<2, false>; break;
+    case 5: kern = residual_bwd_kernel<2, true>; break;
+    case 6: kern = residual_bwd_kernel<3, false>; break;
+    case 7: kern = residual_bwd_kernel<3, true>; break;
+    case 8: kern = residual_bwd_kernel<4, false>; break;
+    default: kern = residual_bwd_kernel<4, true>; break;
   }
-  if (int rc = check_cuda(cudaGetLastError(), "residual_bwd launch")) return rc;
+  const int sum_bytes = sums && vpt > 1 ? static_cast<int>(K) * 12 : 0;
+  if (sum_bytes > 48 * 1024) {
+    if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sum_bytes),
+                            "cudaFuncSetAttribute(residual_bwd)"))
+      return rc;
+  }
+  if (int rc = launch_overlapped(kern, grid, static_cast<unsigned>(threads), static_cast<size_t>(sum_bytes), s, 1, "residual_bwd launch", p))
+    return rc;
   if (!sums) return K2Q_OK;
   SumParams q{};
   q.part = p.part; q.chunks = p.chunks; q.B = B; q.K = p.K; q.normw = norm_scale; q.mscale = p.mscale;
