@@ -109,12 +109,22 @@ __device__ __forceinline__ void norm_mod8(const ResParams& p, int64_t b, int k0,
 
 // ---- sampling: rotated int8 codes -------------------------------------------------------------
 // A CTA works through consecutive rows of one sample.  Its vectors are combined once, in shared memory:
-//   f = (1 + w)(1 + sc) c,  s = sh c   (fp32; c the rotation's normalisation, which commutes with it)  and the gate,
-// so that a row costs one packed bf16 multiply-add per two elements for the stream and one packed fp32 one for h.  Four
+//   f = (1 + w)(1 + sc) in fp32,  sh and the gate in bf16 (the rotation's normalisation enters the scale alone),
+// so that a row costs one packed bf16 multiply-add per two elements for the stream and one packed fp32 one for h.  In
+// odd 128-blocks f's 16-byte pieces are swapped pairwise (the bf16 vectors' four apart), so that the eight lanes of a read
+// phase, which span two blocks, meet all banks.  Four
 // neighbouring lanes hold a 128-block.  Lane q of the four owns the 8-element chunks q, q + 4, q + 8, q + 12 of the
-// block: a warp's 16-byte accesses then cover whole 64-byte pieces (32-byte pieces of the codes), and nothing has to be
-// staged through shared memory.  Of the rotation's seven butterfly stages, h = 1, 2, 4 and 32, 64 lie inside a thread,
-// h = 8 and 16 between lanes.  The next row is requested before the current one is worked on.
+// block: a warp's 16-byte accesses then cover whole 64-byte pieces, and nothing has to be staged through shared memory.
+// The next row is requested before the current one is worked on.
+//
+// The rotation's seven butterfly stages: h = 1, 2, 4 and 32, 64 lie inside a thread, h = 8 and 16 between lanes.  A lane
+// would have to fetch all 32 of its partner's values for each of the latter.  Instead, after stage 32, lane bit 0 and
+// the chunk's low bit change places: of each butterfly's two results the lane keeps the one whose index bit 5 is its
+// own lane bit and sends the other, 16 values; stage 8 then lies inside the thread.  Likewise 64 and 16 with the
+// other bits.  In the end lane q holds the 32 consecutive elements from 32 q on.  The differences of stage 8 (16) come out
+// negated in lanes with bit 0 (1) set; the caller undoes it: rotated_sign().
+__device__ __forceinline__ float rotated_sign(int chunk, int q) { return __popc(chunk & q) & 1 ? -1.0f : 1.0f; }
+
 __device__ __forceinline__ void fwht128_chunks(uint64_t (&p)[16], int q) {
   const uint64_t neg2 = pack_f32x2(-1.0f, -1.0f);
 #pragma unroll
@@ -135,25 +145,25 @@ __device__ __forceinline__ void fwht128_chunks(uint64_t (&p)[16], int q) {
     }
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const float sgn = ((q >> j) & 1) ? -1.0f : 1.0f;     // lower lane a + b, upper lane a - b
-    const uint64_t sgn2 = pack_f32x2(sgn, sgn);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float a, b;
-      unpack_f32x2(p[i], a, b);
-      const float oa = __shfl_xor_sync(0xffffffffu, a, 1 << j), ob = __shfl_xor_sync(0xffffffffu, b, 1 << j);
-      p[i] = fma_f32x2(p[i], sgn2, pack_f32x2(oa, ob));
-    }
-  }
-#pragma unroll
-  for (int h = 4; h < 16; h <<= 1) {
+  for (int h = 4; h < 16; h <<= 1) {                     // 32 and 8, then 64 and 16
+    const float sgn = (q & (h >> 2)) ? -1.0f : 1.0f;
+    const uint64_t sgn2 = pack_f32x2(sgn, sgn), nsgn2 = pack_f32x2(-sgn, -sgn);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       if ((i & h) == 0) {
-        const uint64_t a = p[i], b = p[i + h];
-        p[i] = add_f32x2(a, b);
-        p[i + h] = fma_f32x2(b, neg2, a);
+        const uint64_t keep = fma_f32x2(p[i + h], sgn2, p[i]), send = fma_f32x2(p[i + h], nsgn2, p[i]);
+        float a, b;
+        unpack_f32x2(send, a, b);
+        p[i] = keep;
+        p[i + h] = pack_f32x2(__shfl_xor_sync(0xffffffffu, a, h >> 2), __shfl_xor_sync(0xffffffffu, b, h >> 2));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if ((i & h) == 0) {
+        const uint64_t keep = p[i], got = p[i + h];
+        p[i] = add_f32x2(keep, got);
+        p[i + h] = fma_f32x2(got, neg2, keep);
       }
     }
   }
@@ -167,6 +177,8 @@ __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t 
 }
 __device__ __forceinline__ uint64_t widen2(uint32_t w) { return pack_f32x2(w << 16, w & 0xFFFF0000u); }
 
+constexpr int kQuantRegs = 96;
+
 struct RowChunks { uint4 x[4], y[4]; };
 
 // rows [r0, r1) of sample b that CTA blockIdx.x = b * chunks + chunk works on
@@ -178,11 +190,11 @@ __device__ __forceinline__ void cta_rows(const ResParams& p, int64_t& b, int64_t
 }
 
 template <bool GATE, bool SHIFT>
-__global__ void __launch_bounds__(512) residual_quant_kernel(const ResParams p) {
-  extern __shared__ __align__(16) float vec[];                 // f [K] | s [K] (SHIFT) | gate [K] bf16 (GATE)
+__global__ void __maxnreg__(96) residual_quant_kernel(const ResParams p) {
+  extern __shared__ __align__(16) float vec[];                 // f [K] | sh [K] bf16 (SHIFT) | gate [K] bf16 (GATE)
   __shared__ float red[2][kMaxWarps];
-  float* s_s = vec + p.K;
-  const uint32_t* s_g = reinterpret_cast<const uint32_t*>(vec + (SHIFT ? 2 : 1) * p.K);
+  uint32_t* s_s = reinterpret_cast<uint32_t*>(vec + p.K);
+  uint32_t* s_g = s_s + (SHIFT ? p.K / 2 : 0);
   const int warps = blockDim.x >> 5;
   const int q = threadIdx.x & 3;
   const int blk = threadIdx.x >> 2;                            // 128-block of the row
@@ -211,26 +223,24 @@ __global__ void __launch_bounds__(512) residual_quant_kernel(const ResParams p) 
     float f[8];
     load8f(p.normw + k, f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = (1.0f + f[e]) * kHadNorm;
+    for (int e = 0; e < 8; ++e) f[e] += 1.0f;
     if (p.mscale != nullptr) {
       float s[8];
       unpack8(load_vec16(p.mscale + b * p.K + k), s);
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] *= 1.0f + s[e];
     }
-    *reinterpret_cast<float4*>(vec + k) = make_float4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<float4*>(vec + k + 4) = make_float4(f[4], f[5], f[6], f[7]);
-    if (SHIFT) {
-      float s[8];
-      unpack8(load_vec16(p.mshift + b * p.K + k), s);
-      *reinterpret_cast<float4*>(s_s + k) = make_float4(s[0] * kHadNorm, s[1] * kHadNorm, s[2] * kHadNorm, s[3] * kHadNorm);
-      *reinterpret_cast<float4*>(s_s + k + 4) = make_float4(s[4] * kHadNorm, s[5] * kHadNorm, s[6] * kHadNorm, s[7] * kHadNorm);
-    }
-    if (GATE) *reinterpret_cast<uint4*>(vec + (SHIFT ? 2 : 1) * p.K + (k >> 1)) = load_vec16(p.gate + b * p.K + k);
+    const int swap = (k >> 7) & 1, lo = k + 4 * swap, hi = k + 4 * (swap ^ 1);
+    *reinterpret_cast<float4*>(vec + lo) = make_float4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<float4*>(vec + hi) = make_float4(f[4], f[5], f[6], f[7]);
+    const int at = (k ^ (32 * swap)) >> 1;
+    if (SHIFT) *reinterpret_cast<uint4*>(s_s + at) = load_vec16(p.mshift + b * p.K + k);
+    if (GATE) *reinterpret_cast<uint4*>(s_g + at) = load_vec16(p.gate + b * p.K + k);
   }
   __syncthreads();
 
   const float inv_k = 1.0f / static_cast<float>(p.K);
+  const int lo = k00 + 4 * (blk & 1), hi = k00 + 4 * ((blk & 1) ^ 1);
   for (int64_t row = r0; row < r1; ++row) {
     uint64_t v[16];
     uint64_t ss2[2] = {0ull, 0ull};
@@ -239,7 +249,7 @@ __global__ void __launch_bounds__(512) residual_quant_kernel(const ResParams p) 
       uint4 s = next.x[j];
       const uint4 y = next.y[j];
       uint4 g = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u);   // one
-      if (GATE && own) g = *reinterpret_cast<const uint4*>(s_g + ((k00 + 32 * j) >> 1));
+      if (GATE && own) g = *reinterpret_cast<const uint4*>(s_g + ((k00 + 32 * (j ^ (blk & 1))) >> 1));
       s.x = fma_bf16x2(g.x, y.x, s.x); s.y = fma_bf16x2(g.y, y.y, s.y);
       s.z = fma_bf16x2(g.z, y.z, s.z); s.w = fma_bf16x2(g.w, y.w, s.w);
       if (own) *reinterpret_cast<uint4*>(p.stream + row * p.lds + k00 + 32 * j) = s;
@@ -256,11 +266,11 @@ __global__ void __launch_bounds__(512) residual_quant_kernel(const ResParams p) 
     if (own) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const ulonglong2 f0 = *reinterpret_cast<const ulonglong2*>(vec + k00 + 32 * j), f1 = *reinterpret_cast<const ulonglong2*>(vec + k00 + 32 * j + 4);
+        const ulonglong2 f0 = *reinterpret_cast<const ulonglong2*>(vec + lo + 32 * j), f1 = *reinterpret_cast<const ulonglong2*>(vec + hi + 32 * j);
         const uint64_t f[4] = {f0.x, f0.y, f1.x, f1.y};
         if (SHIFT) {
-          const ulonglong2 s0 = *reinterpret_cast<const ulonglong2*>(s_s + k00 + 32 * j), s1 = *reinterpret_cast<const ulonglong2*>(s_s + k00 + 32 * j + 4);
-          const uint64_t s[4] = {s0.x, s0.y, s1.x, s1.y};
+          const uint4 sv = *reinterpret_cast<const uint4*>(s_s + ((k00 + 32 * (j ^ (blk & 1))) >> 1));
+          const uint64_t s[4] = {widen2(sv.x), widen2(sv.y), widen2(sv.z), widen2(sv.w)};
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[4 * j + e] = fma_f32x2(mul_f32x2(v[4 * j + e], rstd2), f[e], s[e]);
         } else {
@@ -278,22 +288,25 @@ __global__ void __launch_bounds__(512) residual_quant_kernel(const ResParams p) 
       m0 = max_nan(m0, fabsf(a));
       m1 = max_nan(m1, fabsf(c));
     }
-    const float s = __fdiv_rn(max_nan(cta_reduce<true>(max_nan(m0, m1), red[1], warps), 1e-8f), 127.0f);
-    const float inv = __frcp_rn(s);
+    // the scale of the normalised rotation; codes straight from the values without its factor
+    const float s = __fdiv_rn(max_nan(cta_reduce<true>(max_nan(m0, m1), red[1], warps) * kHadNorm, 1e-8f), 127.0f);
+    const float inv = __fdividef(kHadNorm, s);
     // v / s + 1.5 * 2^23 carries the rounded code in its low byte
-    const uint64_t inv2 = pack_f32x2(inv, inv), magic2 = pack_f32x2(kRoundMagic, kRoundMagic);
+    const uint64_t magic2 = pack_f32x2(kRoundMagic, kRoundMagic);
     uint32_t words[8];
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
+      const float signed_inv = inv * rotated_sign(w >> 1, q);
+      const uint64_t inv2 = pack_f32x2(signed_inv, signed_inv);
       float c0, c1, c2, c3;
       unpack_f32x2(fma_f32x2(v[2 * w], inv2, magic2), c0, c1);
       unpack_f32x2(fma_f32x2(v[2 * w + 1], inv2, magic2), c2, c3);
       words[w] = prmt_b(prmt_b(__float_as_uint(c0), __float_as_uint(c1), 0x0040u), prmt_b(__float_as_uint(c2), __float_as_uint(c3), 0x0040u), 0x5410u);
     }
     if (own) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<uint2*>(p.xq + row * p.K + k00 + 32 * j) = make_uint2(words[2 * j], words[2 * j + 1]);
+      uint4* out = reinterpret_cast<uint4*>(p.xq + row * p.K + blk * 128 + q * 32);
+      out[0] = make_uint4(words[0], words[1], words[2], words[3]);
+      out[1] = make_uint4(words[4], words[5], words[6], words[7]);
     }
     if (threadIdx.x == 0) p.sx[row] = s;
   }
@@ -622,20 +635,21 @@ int k2q_residual_norm_quant(const void* x_bf16, int64_t ldx, const void* y_bf16,
     return fail(K2Q_EINVAL, "%s: rows must be 16-byte aligned with a leading dimension >= K", name);
   const int threads = (static_cast<int>(K / 32) + 31) / 32 * 32;
   const int64_t B = M / rows_per_batch;
-  // registers let about 640 threads share an SM, the vectors in shared memory must fit as often
-  const int vec_bytes = static_cast<int>(K) * (4 + (p.mshift ? 4 : 0) + (p.gate ? 2 : 0));
-  int ctas = threads >= 640 ? 1 : 640 / threads;
-  if (ctas > 220 * 1024 / (vec_bytes + 1024)) ctas = 220 * 1024 / (vec_bytes + 1024);
+  // CTAs per SM: a quarter of an SM's registers holds 512 / kQuantRegs warps, and the vectors must fit as often
+  const int vec_bytes = static_cast<int>(K) * (4 + (p.mshift ? 2 : 0) + (p.gate ? 2 : 0));
+  int ctas = 4 * (512 / kQuantRegs) / (threads / 32);
+  if (ctas > 224 * 1024 / (vec_bytes + 1280)) ctas = 224 * 1024 / (vec_bytes + 1280);
   if (ctas > 16) ctas = 16;
   p.chunks = chunks_for(B, rows_per_batch, ctas < 1 ? 1 : ctas);
   if (B * p.chunks > 0x7fffffffLL) return fail(K2Q_EINVAL, "%s: too many samples (%lld)", name, (long long)B);
   auto kern = p.gate ? (p.mshift ? residual_quant_kernel<true, true> : residual_quant_kernel<true, false>)
                      : (p.mshift ? residual_quant_kernel<false, true> : residual_quant_kernel<false, false>);
-  if (vec_bytes > 48 * 1024) {
-    if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, vec_bytes),
-                            "cudaFuncSetAttribute(residual_quant)"))
-      return rc;
-  }
+  if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, vec_bytes),
+                          "cudaFuncSetAttribute(residual_quant)"))
+    return rc;
+  if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared),
+                          "cudaFuncSetAttribute(residual_quant)"))
+    return rc;
   return launch_overlapped(kern, static_cast<unsigned>(B * p.chunks), static_cast<unsigned>(threads), static_cast<size_t>(vec_bytes),
                            static_cast<cudaStream_t>(stream), 1, "residual_quant launch", p);
 }
