@@ -14,6 +14,8 @@
 // Everything between the loads and the stores is fp32; the stream is rounded to bf16 once, where it is
 // kept, and the norm reads the rounded values, so that the backward sees the same numbers.  b = row /
 // rows_per_batch.  All three are bound by HBM: 7, 8 and 8 (10 with the sums) bytes per element.
+#include <atomic>
+
 #include "k2q_common.cuh"
 #include "rows_math.cuh"
 
@@ -46,6 +48,12 @@ __device__ __forceinline__ uint4 load_vec16(const __nv_bfloat16* p) { return __l
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -285,8 +293,8 @@ __global__ void __maxnreg__(96) residual_quant_kernel(const ResParams p) {
     for (int i = 0; i < 16; ++i) {
       float a, c;
       unpack_f32x2(v[i], a, c);
-      m0 = max_nan(m0, fabsf(a));
-      m1 = max_nan(m1, fabsf(c));
+      if (i & 1) m1 = max_abs3(m1, a, c);
+      else m0 = max_abs3(m0, a, c);
     }
     // the scale of the normalised rotation; codes straight from the values without its factor
     const float s = __fdiv_rn(max_nan(cta_reduce<true>(max_nan(m0, m1), red[1], warps) * kHadNorm, 1e-8f), 127.0f);
@@ -538,43 +546,59 @@ struct SumParams {
   const float* normw; const __nv_bfloat16* mscale;
   __nv_bfloat16* dgate; __nv_bfloat16* dmscale; __nv_bfloat16* dmshift;   // [B, K] or NULL
   float* dnorm;                                                           // [K] or NULL
+  float* share;                                                           // [B, K]: a sample's part of dnorm (B > 1)
 };
 
-// 32 columns per CTA; eight groups of threads take every eighth chunk of a sample, and their sums are added
-// in group order: the result does not depend on how the CTAs before were scheduled.
-__global__ void __launch_bounds__(256) residual_sums_kernel(const SumParams p) {
-  __shared__ float s[8][3][32];
+// 32 columns of one sample per CTA; sixteen groups of threads take every sixteenth chunk, and their sums are added in
+// group order: the result does not depend on how the CTAs before were scheduled.
+constexpr int kSumGroups = 16;
+__global__ void __launch_bounds__(32 * kSumGroups) residual_sums_kernel(const SumParams p) {
+  __shared__ float s[kSumGroups][3][32];
   const int col = threadIdx.x & 31, grp = threadIdx.x >> 5;
   const int k = blockIdx.x * 32 + col;
+  const int64_t b = blockIdx.y;
   const bool ok = k < p.K;
-  float dn = 0.f;
-  for (int64_t b = 0; b < p.B; ++b) {
-    float a[3] = {0.f, 0.f, 0.f};
-    if (ok) {
-      for (int c = grp; c < p.chunks; c += 8) {
-        const float* src = p.part + ((b * p.chunks + c) * 3) * p.K + k;
-        a[0] += src[0];
-        a[1] += src[p.K];
-        a[2] += src[2 * static_cast<int64_t>(p.K)];
-      }
-    }
-    __syncthreads();                        // the previous sample's sums have been read
-#pragma unroll
-    for (int j = 0; j < 3; ++j) s[grp][j][col] = a[j];
-    __syncthreads();
-    if (grp == 0 && ok) {
-#pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        a[j] = s[0][j][col];
-        for (int g = 1; g < 8; ++g) a[j] += s[g][j][col];
-      }
-      if (p.dgate != nullptr) p.dgate[b * p.K + k] = __float2bfloat16_rn(a[0]);
-      if (p.dmscale != nullptr) p.dmscale[b * p.K + k] = __float2bfloat16_rn(a[1] * (1.0f + p.normw[k]));
-      if (p.dmshift != nullptr) p.dmshift[b * p.K + k] = __float2bfloat16_rn(a[2]);
-      dn += p.mscale != nullptr ? a[1] * (1.0f + __bfloat162float(p.mscale[b * p.K + k])) : a[1];
+  pdl_wait();
+  float a[3] = {0.f, 0.f, 0.f};
+  if (ok) {
+#pragma unroll 4
+    for (int c = grp; c < p.chunks; c += kSumGroups) {
+      const float* src = p.part + ((b * p.chunks + c) * 3) * p.K + k;
+      a[0] += src[0];
+      a[1] += src[p.K];
+      a[2] += src[2 * static_cast<int64_t>(p.K)];
     }
   }
-  if (grp == 0 && ok && p.dnorm != nullptr) p.dnorm[k] = dn;
+#pragma unroll
+  for (int j = 0; j < 3; ++j) s[grp][j][col] = a[j];
+  __syncthreads();
+  if (grp == 0 && ok) {
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      a[j] = s[0][j][col];
+#pragma unroll
+      for (int g = 1; g < kSumGroups; ++g) a[j] += s[g][j][col];
+    }
+    const int64_t at = b * p.K + k;
+    if (p.dgate != nullptr) p.dgate[at] = __float2bfloat16_rn(a[0]);
+    if (p.dmscale != nullptr) p.dmscale[at] = __float2bfloat16_rn(a[1] * (1.0f + p.normw[k]));
+    if (p.dmshift != nullptr) p.dmshift[at] = __float2bfloat16_rn(a[2]);
+    if (p.dnorm != nullptr) {
+      const float d = p.mscale != nullptr ? a[1] * (1.0f + __bfloat162float(p.mscale[at])) : a[1];
+      if (p.B == 1) p.dnorm[k] = d;
+      else p.share[at] = d;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(128) residual_dnorm_kernel(const SumParams p) {
+  const int k = blockIdx.x * 128 + threadIdx.x;
+  pdl_wait();
+  if (k >= p.K) return;
+  float d = 0.f;
+#pragma unroll 8
+  for (int64_t b = 0; b < p.B; ++b) d += p.share[b * p.K + k];
+  p.dnorm[k] = d;
 }
 
 // ---- host side ------------------------------------------------------------------------------------
@@ -598,14 +622,46 @@ int chunks_for(int64_t B, int64_t rows_per_batch, int ctas_per_sm) {
   if (c > rows_per_batch) c = rows_per_batch;
   return static_cast<int>(c < 1 ? 1 : c);
 }
-// CTAs of the dense kernels that share an SM: about 768 threads
-int dense_ctas(int threads) { return threads >= 512 ? 1 : 768 / threads; }
+using Kernel = void (*)(ResParams);
+// CTAs of a kernel that share an SM, asked of the runtime once per kernel (`slot`) and number of warps
+int ctas_per_sm(Kernel kern, int slot, int threads, int smem) {
+  static std::atomic<int> known[16][17];
+  std::atomic<int>& k = known[slot][threads / 32];
+  int n = k.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, static_cast<size_t>(smem)) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      return 1;
+    }
+    k.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
 
 // threads per CTA and 16-byte vectors per thread of the dense kernels
 void dense_shape(int64_t K, int* threads, int* vpt) {
   const int nvec = static_cast<int>(K / 8);
   *vpt = (nvec + 511) / 512;
   *threads = ((nvec + *vpt - 1) / *vpt + 31) / 32 * 32;
+}
+
+const Kernel kQuant[4] = {residual_quant_kernel<false, false>, residual_quant_kernel<false, true>, residual_quant_kernel<true, false>,
+                          residual_quant_kernel<true, true>};
+const Kernel kFwd[4] = {residual_fwd_kernel<1>, residual_fwd_kernel<2>, residual_fwd_kernel<3>, residual_fwd_kernel<4>};
+const Kernel kBwd[8] = {residual_bwd_kernel<1, false>, residual_bwd_kernel<1, true>, residual_bwd_kernel<2, false>,
+                        residual_bwd_kernel<2, true>,  residual_bwd_kernel<3, false>, residual_bwd_kernel<3, true>,
+                        residual_bwd_kernel<4, false>, residual_bwd_kernel<4, true>};
+
+struct BwdShape { int threads, slot, smem, chunks; };
+BwdShape bwd_shape(int64_t B, int64_t rows_per_batch, int64_t K, bool sums) {
+  BwdShape s{};
+  int vpt;
+  dense_shape(K, &s.threads, &vpt);
+  s.slot = (vpt - 1) * 2 + (sums ? 1 : 0);
+  s.smem = sums && vpt > 1 ? static_cast<int>(K) * 12 : 0;
+  s.chunks = chunks_for(B, rows_per_batch, ctas_per_sm(kBwd[s.slot], s.slot, s.threads, s.smem));
+  return s;
 }
 
 }  // namespace
@@ -635,22 +691,14 @@ int k2q_residual_norm_quant(const void* x_bf16, int64_t ldx, const void* y_bf16,
     return fail(K2Q_EINVAL, "%s: rows must be 16-byte aligned with a leading dimension >= K", name);
   const int threads = (static_cast<int>(K / 32) + 31) / 32 * 32;
   const int64_t B = M / rows_per_batch;
-  // CTAs per SM: a quarter of an SM's registers holds 512 / kQuantRegs warps, and the vectors must fit as often
   const int vec_bytes = static_cast<int>(K) * (4 + (p.mshift ? 2 : 0) + (p.gate ? 2 : 0));
-  int ctas = 4 * (512 / kQuantRegs) / (threads / 32);
-  if (ctas > 224 * 1024 / (vec_bytes + 1280)) ctas = 224 * 1024 / (vec_bytes + 1280);
-  if (ctas > 16) ctas = 16;
-  p.chunks = chunks_for(B, rows_per_batch, ctas < 1 ? 1 : ctas);
+  const int slot = (p.gate ? 2 : 0) + (p.mshift ? 1 : 0);
+  p.chunks = chunks_for(B, rows_per_batch, ctas_per_sm(kQuant[slot], 12 + slot, threads, vec_bytes));
   if (B * p.chunks > 0x7fffffffLL) return fail(K2Q_EINVAL, "%s: too many samples (%lld)", name, (long long)B);
-  auto kern = p.gate ? (p.mshift ? residual_quant_kernel<true, true> : residual_quant_kernel<true, false>)
-                     : (p.mshift ? residual_quant_kernel<false, true> : residual_quant_kernel<false, false>);
-  if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, vec_bytes),
+  if (int rc = check_cuda(cudaFuncSetAttribute(kQuant[slot], cudaFuncAttributeMaxDynamicSharedMemorySize, vec_bytes),
                           "cudaFuncSetAttribute(residual_quant)"))
     return rc;
-  if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared),
-                          "cudaFuncSetAttribute(residual_quant)"))
-    return rc;
-  return launch_overlapped(kern, static_cast<unsigned>(B * p.chunks), static_cast<unsigned>(threads), static_cast<size_t>(vec_bytes),
+  return launch_overlapped(kQuant[slot], static_cast<unsigned>(B * p.chunks), static_cast<unsigned>(threads), static_cast<size_t>(vec_bytes),
                            static_cast<cudaStream_t>(stream), 1, "residual_quant launch", p);
 }
 
@@ -676,23 +724,16 @@ int k2q_residual_norm_fwd(const void* x_bf16, int64_t ldx, const void* y_bf16, i
   int threads, vpt;
   dense_shape(K, &threads, &vpt);
   const int64_t B = M / rows_per_batch;
-  p.chunks = chunks_for(B, rows_per_batch, dense_ctas(threads));
+  p.chunks = chunks_for(B, rows_per_batch, ctas_per_sm(kFwd[vpt - 1], 8 + vpt - 1, threads, 0));
   if (B * p.chunks > 0x7fffffffLL) return fail(K2Q_EINVAL, "%s: too many samples (%lld)", name, (long long)B);
-  auto kern = vpt == 1 ? residual_fwd_kernel<1> : vpt == 2 ? residual_fwd_kernel<2> : vpt == 3 ? residual_fwd_kernel<3> : residual_fwd_kernel<4>;
-  return launch_overlapped(kern, static_cast<unsigned>(B * p.chunks), static_cast<unsigned>(threads), 0, static_cast<cudaStream_t>(stream), 1,
-                           "residual_fwd launch", p);
-}
-
-static int bwd_chunks(int64_t B, int64_t rows_per_batch, int64_t K) {
-  int threads, vpt;
-  dense_shape(K, &threads, &vpt);
-  return chunks_for(B, rows_per_batch, dense_ctas(threads));
+  return launch_overlapped(kFwd[vpt - 1], static_cast<unsigned>(B * p.chunks), static_cast<unsigned>(threads), 0,
+                           static_cast<cudaStream_t>(stream), 1, "residual_fwd launch", p);
 }
 
 int64_t k2q_residual_norm_bwd_workspace_bytes(int64_t rows_per_batch, int64_t M, int64_t K) {
-  if (rows_per_batch <= 0 || M <= 0 || K <= 0) return 0;
+  if (rows_per_batch <= 0 || M <= 0 || K <= 0 || K > 16384) return 0;
   const int64_t B = M / rows_per_batch;
-  return B * bwd_chunks(B, rows_per_batch, K) * 3 * K * static_cast<int64_t>(sizeof(float));
+  return (B * bwd_shape(B, rows_per_batch, K, true).chunks * 3 + (B > 1 ? B : 0)) * K * static_cast<int64_t>(sizeof(float));
 }
 
 int k2q_residual_norm_bwd(const void* dstream_bf16, int64_t ldds, const void* dh_bf16, int64_t lddh,
@@ -723,7 +764,8 @@ int k2q_residual_norm_bwd(const void* dstream_bf16, int64_t ldds, const void* dh
   if (dgate_bf16 && (!p.gate || !p.y)) return fail(K2Q_EINVAL, "%s: the gate's gradient needs gate and y", name);
   const int64_t B = M / rows_per_batch;
   const bool sums = dgate_bf16 || dmod_scale_bf16 || dmod_shift_bf16 || dnorm;
-  p.chunks = bwd_chunks(B, rows_per_batch, K);
+  const BwdShape shape = bwd_shape(B, rows_per_batch, K, sums);
+  p.chunks = shape.chunks;
   if (!dgate_bf16) p.y = nullptr;
   if (sums) {
     if (!ws || off16(ws) || ws_bytes < k2q_residual_norm_bwd_workspace_bytes(rows_per_batch, M, K))
@@ -731,36 +773,34 @@ int k2q_residual_norm_bwd(const void* dstream_bf16, int64_t ldds, const void* dh
     p.part = static_cast<float*>(ws);
   }
   if (B * p.chunks > 0x7fffffffLL) return fail(K2Q_EINVAL, "%s: too many samples (%lld)", name, (long long)B);
-  int threads, vpt;
-  dense_shape(K, &threads, &vpt);
+  if (sums && (B > 65535)) return fail(K2Q_EINVAL, "%s: sums over the rows of more than 65535 samples", name);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = static_cast<unsigned>(B * p.chunks);
-  void (*kern)(ResParams) = nullptr;
-  switch (vpt * 2 + (sums ? 1 : 0)) {
-    case 2: kern = residual_bwd_kernel<1, false>; break;
-    case 3: kern = residual_bwd_kernel<1, true>; break;
-    case 4: kern = residual_bwd_kernel<2, false>; break;
-    case 5: kern = residual_bwd_kernel<2, true>; break;
-    case 6: kern = residual_bwd_kernel<3, false>; break;
-    case 7: kern = residual_bwd_kernel<3, true>; break;
-    case 8: kern = residual_bwd_kernel<4, false>; break;
-    default: kern = residual_bwd_kernel<4, true>; break;
-  }
-  const int sum_bytes = sums && vpt > 1 ? static_cast<int>(K) * 12 : 0;
-  if (sum_bytes > 48 * 1024) {
-    if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sum_bytes),
+  if (shape.smem > 0) {
+    if (int rc = check_cuda(cudaFuncSetAttribute(kBwd[shape.slot], cudaFuncAttributeMaxDynamicSharedMemorySize, shape.smem),
                             "cudaFuncSetAttribute(residual_bwd)"))
       return rc;
   }
-  if (int rc = launch_overlapped(kern, grid, static_cast<unsigned>(threads), static_cast<size_t>(sum_bytes), s, 1, "residual_bwd launch", p))
+  if (int rc = launch_overlapped(kBwd[shape.slot], static_cast<unsigned>(B * p.chunks), static_cast<unsigned>(shape.threads),
+                                 static_cast<size_t>(shape.smem), s, 1, "residual_bwd launch", p))
     return rc;
   if (!sums) return K2Q_OK;
   SumParams q{};
   q.part = p.part; q.chunks = p.chunks; q.B = B; q.K = p.K; q.normw = norm_scale; q.mscale = p.mscale;
   q.dgate = static_cast<__nv_bfloat16*>(dgate_bf16); q.dmscale = static_cast<__nv_bfloat16*>(dmod_scale_bf16);
   q.dmshift = static_cast<__nv_bfloat16*>(dmod_shift_bf16); q.dnorm = dnorm;
-  residual_sums_kernel<<<(p.K + 31) / 32, 256, 0, s>>>(q);
-  return check_cuda(cudaGetLastError(), "residual_sums launch");
+  q.share = p.part + B * p.chunks * 3 * static_cast<int64_t>(p.K);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((p.K + 31) / 32), static_cast<unsigned>(B));
+  cfg.blockDim = dim3(32 * kSumGroups);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = overlapped_launch_allowed(s) ? 1 : 0;
+  if (int rc = check_cuda(cudaLaunchKernelEx(&cfg, residual_sums_kernel, q), "residual_sums launch")) return rc;
+  if (!dnorm || B == 1) return K2Q_OK;
+  return launch_overlapped(residual_dnorm_kernel, static_cast<unsigned>((p.K + 127) / 128), 128u, 0, s, 1, "residual_dnorm launch", q);
 }
 
 }  // extern "C"
