@@ -185,7 +185,7 @@ __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t 
 }
 __device__ __forceinline__ uint64_t widen2(uint32_t w) { return pack_f32x2(w << 16, w & 0xFFFF0000u); }
 
-constexpr int kQuantRegs = 96;
+
 
 struct RowChunks { uint4 x[4], y[4]; };
 
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(512) residual_fwd_kernel(const ResParams p) {
   int it = 0;
   for (int64_t row = r0; row < r1; ++row, it ^= 1) {
     uint4 sv[VPT];
-    float ss = 0.f;
+    uint64_t ss2 = 0ull;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
@@ -357,12 +357,14 @@ __global__ void __launch_bounds__(512) residual_fwd_kernel(const ResParams p) {
         s.z = fma_bf16x2(g.z, ny[i].z, s.z); s.w = fma_bf16x2(g.w, ny[i].w, s.w);
         reinterpret_cast<uint4*>(p.stream + row * p.lds)[c] = s;
         sv[i] = s;
-        float v[8];
-        unpack8(s, v);
+        const uint64_t v[4] = {widen2(s.x), widen2(s.y), widen2(s.z), widen2(s.w)};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
+        for (int e = 0; e < 4; ++e) ss2 = fma_f32x2(v[e], v[e], ss2);
       }
     }
+    float ss, ss_odd;
+    unpack_f32x2(ss2, ss, ss_odd);
+    ss += ss_odd;
     if (row + 1 < r1) fetch(row + 1);
     const float rstd = rsqrtf(cta_reduce<false>(ss, red[it], warps) / static_cast<float>(p.K) + p.eps);
     if (threadIdx.x == 0) p.rstd[row] = rstd;
@@ -384,7 +386,7 @@ __global__ void __launch_bounds__(512) residual_fwd_kernel(const ResParams p) {
 // Up to two vectors per thread the next row is requested before the current one is worked on, and the sample's
 // (1 + w)(1 + sc) stays in registers; beyond, registers hold one row and the vectors are read again (L2).
 template <int VPT, bool SUMS>
-__global__ void __launch_bounds__(512) residual_bwd_kernel(const ResParams p) {
+__global__ void __maxnreg__(VPT == 1 ? (SUMS ? 96 : 64) : VPT == 2 && !SUMS ? 96 : 128) residual_bwd_kernel(const ResParams p) {
   constexpr bool PRE = VPT <= 2, SHARED = SUMS && VPT > 1;
   constexpr int Y = SUMS ? VPT : 1, W = PRE ? VPT : 1, A = SUMS && !SHARED ? 1 : 0;
   extern __shared__ __align__(16) float sums[];                // SHARED: D [K], S [K], H [K]
@@ -394,7 +396,7 @@ __global__ void __launch_bounds__(512) residual_bwd_kernel(const ResParams p) {
   cta_rows(p, b, r0, r1);
   pdl_wait();
   const bool has_h = p.dh != nullptr, has_s = p.dstream != nullptr, sum_d = SUMS && p.y != nullptr;
-  float acc[A ? 3 : 1][8] = {};
+  uint64_t acc[A ? 3 : 1][4] = {};
   uint4 n_ds[VPT], n_dh[VPT], n_st[VPT], n_y[Y];
   float n_rstd = 0.f;
 #pragma unroll
@@ -416,19 +418,22 @@ __global__ void __launch_bounds__(512) residual_bwd_kernel(const ResParams p) {
       }
     }
   };
-  auto weights = [&](int c, float* w) {
-    load8f(p.normw + 8 * c, w);
+  auto weights = [&](int c, uint64_t* w) {
+    float f[8];
+    load8f(p.normw + 8 * c, f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] += 1.0f;
+    for (int e = 0; e < 8; ++e) f[e] += 1.0f;
     if (p.mscale != nullptr) {
       float s[8];
       unpack8(load_vec16(p.mscale + b * p.K + 8 * c), s);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] *= 1.0f + s[e];
+      for (int e = 0; e < 8; ++e) f[e] *= 1.0f + s[e];
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pack_f32x2(f[2 * e], f[2 * e + 1]);
   };
   fetch(r0);                                                   // chunks <= rows_per_batch: there is a row
-  float w_keep[W][8];
+  uint64_t w_keep[W][4];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
@@ -443,23 +448,28 @@ __global__ void __launch_bounds__(512) residual_bwd_kernel(const ResParams p) {
       }
     }
   }
-  // adds v[e] * u[e] (or v[e] with u NULL) to a sum of this thread's columns 8c ..
-  auto add = [&](int j, int c, const float* v, const float* u) {
+  // sum j of this thread's columns 8c .. += v * u, or + v
+  auto add = [&](int j, int c, const uint64_t* v, const uint64_t* u) {
     if (A) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[A ? j : 0][e] = u != nullptr ? fmaf(v[e], u[e], acc[A ? j : 0][e]) : acc[A ? j : 0][e] + v[e];
+      for (int e = 0; e < 4; ++e) acc[A ? j : 0][e] = u != nullptr ? fma_f32x2(v[e], u[e], acc[A ? j : 0][e]) : add_f32x2(acc[A ? j : 0][e], v[e]);
     } else {
 #pragma unroll
-      for (int h = 0; h < 8; h += 4) {
-        float4* at = reinterpret_cast<float4*>(sums + j * p.K + 8 * c + h);
-        float4 s = *at;
-        s.x = u != nullptr ? fmaf(v[h], u[h], s.x) : s.x + v[h];
-        s.y = u != nullptr ? fmaf(v[h + 1], u[h + 1], s.y) : s.y + v[h + 1];
-        s.z = u != nullptr ? fmaf(v[h + 2], u[h + 2], s.z) : s.z + v[h + 2];
-        s.w = u != nullptr ? fmaf(v[h + 3], u[h + 3], s.w) : s.w + v[h + 3];
+      for (int h = 0; h < 2; ++h) {
+        ulonglong2* at = reinterpret_cast<ulonglong2*>(sums + j * p.K + 8 * c + 4 * h);
+        ulonglong2 s = *at;
+        s.x = u != nullptr ? fma_f32x2(v[2 * h], u[2 * h], s.x) : add_f32x2(s.x, v[2 * h]);
+        s.y = u != nullptr ? fma_f32x2(v[2 * h + 1], u[2 * h + 1], s.y) : add_f32x2(s.y, v[2 * h + 1]);
         *at = s;
       }
     }
+  };
+  auto widen8 = [](const uint4& r, uint64_t* v) { v[0] = widen2(r.x); v[1] = widen2(r.y); v[2] = widen2(r.z); v[3] = widen2(r.w); };
+  auto narrow8 = [](const uint64_t* v) {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) unpack_f32x2(v[e], f[2 * e], f[2 * e + 1]);
+    return pack8(f);
   };
   const float inv_k = 1.0f / static_cast<float>(p.K);
   int it = 0;
@@ -467,58 +477,66 @@ __global__ void __launch_bounds__(512) residual_bwd_kernel(const ResParams p) {
     if (!PRE && row > r0) fetch(row);
     uint4 c_ds[VPT], c_dh[VPT], c_st[VPT], c_y[Y];
     const float rstd = n_rstd;
-    float dot = 0.f;
+    const uint64_t rstd2 = pack_f32x2(rstd, rstd);
+    uint64_t dot2 = 0ull;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
       c_ds[i] = n_ds[i]; c_dh[i] = n_dh[i]; c_st[i] = n_st[i];
       if (SUMS) c_y[SUMS ? i : 0] = n_y[SUMS ? i : 0];
       if (c < nvec) {
-        float g[8], n[8], w[8];
-        unpack8(c_dh[i], g);
-        unpack8(c_st[i], n);
+        uint64_t g[4], n[4], w[4];
+        widen8(c_dh[i], g);
+        widen8(c_st[i], n);
         if (!PRE) weights(c, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) n[e] *= rstd;
+        for (int e = 0; e < 4; ++e) n[e] = mul_f32x2(n[e], rstd2);
         if (SUMS) {
           add(1, c, g, n);
           add(2, c, g, nullptr);
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) dot = fmaf(g[e] * (PRE ? w_keep[PRE ? i : 0][e] : w[e]), n[e], dot);
+        for (int e = 0; e < 4; ++e) dot2 = fma_f32x2(mul_f32x2(g[e], PRE ? w_keep[PRE ? i : 0][e] : w[e]), n[e], dot2);
       }
     }
     if (PRE && row + 1 < r1) fetch(row + 1);
-    if (has_h) dot = cta_reduce<false>(dot, red[it], warps) * inv_k;
+    float dot = 0.f;
+    if (has_h) {
+      float d0, d1;
+      unpack_f32x2(dot2, d0, d1);
+      dot = cta_reduce<false>(d0 + d1, red[it], warps) * inv_k;
+    }
+    const float back = -rstd * dot;                            // n is stream * rstd: n * dot = stream * (rstd dot)
+    const uint64_t back2 = pack_f32x2(back, back);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
       if (c < nvec) {
-        float d[8];
-        unpack8(c_ds[i], d);
+        uint64_t d[4];
+        widen8(c_ds[i], d);
         if (has_h) {
-          float g[8], n[8], w[8];
-          unpack8(c_dh[i], g);
-          unpack8(c_st[i], n);
+          uint64_t g[4], s[4], w[4];
+          widen8(c_dh[i], g);
+          widen8(c_st[i], s);
           if (!PRE) weights(c, w);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            d[e] += rstd * (g[e] * (PRE ? w_keep[PRE ? i : 0][e] : w[e]) - n[e] * rstd * dot);
+          for (int e = 0; e < 4; ++e)
+            d[e] = fma_f32x2(fma_f32x2(s[e], back2, mul_f32x2(g[e], PRE ? w_keep[PRE ? i : 0][e] : w[e])), rstd2, d[e]);
         }
-        if (p.dx != nullptr) __stcs(reinterpret_cast<uint4*>(p.dx + row * p.lddx) + c, pack8(d));
+        if (p.dx != nullptr) __stcs(reinterpret_cast<uint4*>(p.dx + row * p.lddx) + c, narrow8(d));
         if (sum_d) {
-          float y[8];
-          unpack8(c_y[SUMS ? i : 0], y);
+          uint64_t y[4];
+          widen8(c_y[SUMS ? i : 0], y);
           add(0, c, d, y);
         }
         if (p.dy != nullptr) {
           if (p.gate != nullptr) {
-            float gt[8];
-            unpack8(load_vec16(p.gate + b * p.K + 8 * c), gt);
+            uint64_t gt[4];
+            widen8(load_vec16(p.gate + b * p.K + 8 * c), gt);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) d[e] *= gt[e];
+            for (int e = 0; e < 4; ++e) d[e] = mul_f32x2(d[e], gt[e]);
           }
-          __stcs(reinterpret_cast<uint4*>(p.dy + row * p.lddy) + c, pack8(d));
+          __stcs(reinterpret_cast<uint4*>(p.dy + row * p.lddy) + c, narrow8(d));
         }
       }
     }
@@ -532,10 +550,10 @@ __global__ void __launch_bounds__(512) residual_bwd_kernel(const ResParams p) {
 #pragma unroll
         for (int j = 0; j < 3; ++j)
 #pragma unroll
-          for (int h = 0; h < 8; h += 4)
-            *reinterpret_cast<float4*>(part + j * p.K + 8 * c + h) =
-                SHARED ? *reinterpret_cast<const float4*>(sums + j * p.K + 8 * c + h)
-                       : make_float4(acc[A ? j : 0][h], acc[A ? j : 0][h + 1], acc[A ? j : 0][h + 2], acc[A ? j : 0][h + 3]);
+          for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<ulonglong2*>(part + j * p.K + 8 * c + 4 * h) =
+                SHARED ? *reinterpret_cast<const ulonglong2*>(sums + j * p.K + 8 * c + 4 * h)
+                       : make_ulonglong2(acc[A ? j : 0][2 * h], acc[A ? j : 0][2 * h + 1]);
       }
     }
   }
