@@ -23,7 +23,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _aligned_rows, _check_residual, _mod_vec, _ptr, _row_stride, _stream
+from .ops import _check_residual, _launch, _mod_vec, _one_device, _opt_ptr, _ptr, _row_operand
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -39,9 +39,7 @@ def _kernel_ok(*tensors) -> bool:
 
 
 def _call(name: str, dev, *args) -> None:
-    with torch.cuda.device(dev):
-        rc = getattr(_lib.load(), name)(*args, _stream(dev))
-    _lib.check(rc, name)
+    _launch(dev, getattr(_lib.load(), name), name, *args)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -238,23 +236,25 @@ def gate_residual(x: torch.Tensor, gate: torch.Tensor, y: torch.Tensor) -> torch
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, norm_scale, gate, mod_scale, mod_shift, eps):
-        k = x.shape[-1]
+        dev, k = x.device, x.shape[-1]
         m = x.numel() // k
         rows = x.shape[-2] if x.dim() >= 3 else m
         nb = m // rows
-        x2, y2 = _aligned_rows(x), _aligned_rows(y)
+        x2, xp, ldx = _row_operand(x, k)
+        y2, yp, ldy = _row_operand(y, k)
         w = norm_scale if norm_scale.data_ptr() % 16 == 0 else norm_scale.clone()
-        g, sc, sh = (_mod_vec("residual_norm", n, t, nb, k) for n, t in (("gate", gate), ("mod_scale", mod_scale),
-                                                                         ("mod_shift", mod_shift)))
-        stream = torch.empty(m, k, dtype=torch.bfloat16, device=x.device)
-        h = torch.empty(m, k, dtype=torch.bfloat16, device=x.device)
-        rstd = torch.empty(m, dtype=torch.float32, device=x.device)
-        _call("k2q_residual_norm_fwd", x.device, _ptr(x2), _row_stride(x2), _ptr(y2), _row_stride(y2), _ptr(g), _ptr(w),
-              _ptr(sc), _ptr(sh), rows, m, k, float(eps), _ptr(stream), k, _ptr(h), k, _ptr(rstd))
-        stream, h = stream.view(x.shape), h.view(x.shape)
-        ctx.save_for_backward(stream, rstd, w, g, sc, y2 if gate is not None and gate.requires_grad else None)
-        ctx.rows = rows
-        ctx.shapes = tuple(None if t is None else t.shape for t in (x, norm_scale, gate, mod_scale, mod_shift))
+        g = _mod_vec("residual_norm", "gate", gate, nb, k)
+        sc = _mod_vec("residual_norm", "mod_scale", mod_scale, nb, k)
+        sh = _mod_vec("residual_norm", "mod_shift", mod_shift, nb, k)
+        stream = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+        h = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+        rstd = torch.empty(m, dtype=torch.float32, device=dev)
+        _launch(dev, _lib.load().k2q_residual_norm_fwd, "k2q_residual_norm_fwd", xp, ldx, yp, ldy, _opt_ptr(g), w.data_ptr(),
+                _opt_ptr(sc), _opt_ptr(sh), rows, m, k, eps, stream.data_ptr(), k, h.data_ptr(), k, rstd.data_ptr())
+        ctx.save_for_backward(stream, rstd, w, g, sc, y2 if ctx.needs_input_grad[3] else None)
+        ctx.dims = (rows, m, k)
+        ctx.shapes = (x.shape, norm_scale.shape, None if gate is None else gate.shape,
+                      None if mod_scale is None else mod_scale.shape, None if mod_shift is None else mod_shift.shape)
         ctx.set_materialize_grads(False)
         return stream, h
 
@@ -265,43 +265,33 @@ class _ResidualNorm(torch.autograd.Function):
         if ds is None and dh is None:
             return (None,) * 7
         need_x, need_y, need_w, need_g, need_sc, need_sh, _ = ctx.needs_input_grad
-        xs, ws_, gs, scs, shs = ctx.shapes
-        k = xs[-1]
-        m = stream.numel() // k
+        xs, wshape, gs, scs, shs = ctx.shapes
+        rows, m, k = ctx.dims
         dev = stream.device
-        nb = m // ctx.rows
 
         def grad_rows(t):
-            return None if t is None else _aligned_rows(t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16))
+            return (None, 0, 0) if t is None else _row_operand(t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16), k)
 
-        ds2, dh2, s2 = grad_rows(ds), grad_rows(dh), stream.view(m, k)
-        bf = dict(dtype=torch.bfloat16, device=dev)
+        def new(shape, wanted):
+            return torch.empty(shape, dtype=torch.bfloat16, device=dev) if wanted else None
+
+        ds2, dsp, ldds = grad_rows(ds)
+        dh2, dhp, lddh = grad_rows(dh)
+        _, yp, ldy = (None, 0, 0) if y2 is None else _row_operand(y2, k)
         same = g is None                               # without a gate dy equals dx: one tensor serves both
-        dx = torch.empty(m, k, **bf) if need_x or (same and need_y) else None
-        dy = torch.empty(m, k, **bf) if need_y and not same else None
-        dg = torch.empty(nb, k, **bf) if need_g else None
-        dsc = torch.empty(nb, k, **bf) if need_sc else None
-        dsh = torch.empty(nb, k, **bf) if need_sh else None
-        dw = torch.empty(k, dtype=torch.float32, device=dev) if need_w else None
-        ws = None
-        ws_bytes = 0
+        dx = new(xs, need_x or (same and need_y))
+        dy = new(xs, need_y and not same)
+        dg, dsc, dsh = new(gs, need_g), new(scs, need_sc), new(shs, need_sh)
+        dw = torch.empty(wshape, dtype=torch.float32, device=dev) if need_w else None
+        lib = _lib.load()
+        ws, ws_bytes = None, 0
         if need_g or need_sc or need_sh or need_w:
-            ws_bytes = int(_lib.load().k2q_residual_norm_bwd_workspace_bytes(ctx.rows, m, k))
+            ws_bytes = lib.k2q_residual_norm_bwd_workspace_bytes(rows, m, k)
             ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=dev)
-
-        def ld(t):
-            return 0 if t is None else _row_stride(t)
-
-        _call("k2q_residual_norm_bwd", dev, _ptr(ds2), ld(ds2), _ptr(dh2), ld(dh2), _ptr(s2), k, _ptr(rstd), _ptr(y2), ld(y2),
-              _ptr(g), _ptr(w), _ptr(sc), ctx.rows, m, k, _ptr(dx), k, _ptr(dy), k, _ptr(dg), _ptr(dsc), _ptr(dsh), _ptr(dw),
-              _ptr(ws), ws_bytes)
-
-        def like(t, shape):
-            return None if t is None else t.view(shape)
-
-        dxv = like(dx, xs)
-        return (dxv if need_x else None, (dxv if same else like(dy, xs)) if need_y else None, like(dw, ws_), like(dg, gs),
-                like(dsc, scs), like(dsh, shs), None)
+        _launch(dev, lib.k2q_residual_norm_bwd, "k2q_residual_norm_bwd", dsp, ldds, dhp, lddh, stream.data_ptr(), k, rstd.data_ptr(),
+                yp, ldy, _opt_ptr(g), w.data_ptr(), _opt_ptr(sc), rows, m, k, _opt_ptr(dx), k, _opt_ptr(dy), k, _opt_ptr(dg),
+                _opt_ptr(dsc), _opt_ptr(dsh), _opt_ptr(dw), _opt_ptr(ws), ws_bytes)
+        return (dx if need_x else None, (dx if same else dy) if need_y else None, dw, dg, dsc, dsh, None)
 
 
 def residual_norm(x: torch.Tensor, y: torch.Tensor, norm_scale: torch.Tensor, gate: torch.Tensor | None = None,
@@ -313,12 +303,10 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, norm_scale: torch.Tensor, ga
     stream rounded once where it is kept.  Where the kernel does not apply (CPU, other types, K not a
     multiple of 8 or above 16384) the same expression runs op by op."""
     k = x.shape[-1]
-    vectors = (gate, mod_scale, mod_shift)
-    if _kernel_ok(x, y, *vectors) and norm_scale.is_cuda and norm_scale.dtype == torch.float32 and k % 8 == 0 and 0 < k <= 16384 \
-            and x.numel() > 0:
+    if (k % 8 == 0 and 0 < k <= 16384 and x.numel() > 0 and norm_scale.dtype == torch.float32 and norm_scale.is_cuda
+            and _kernel_ok(x, y, gate, mod_scale, mod_shift)):
         _check_residual("residual_norm", x, y, norm_scale, k)
-        if len({t.device for t in (x, y, norm_scale, *vectors) if t is not None}) != 1:
-            raise RuntimeError("residual_norm: tensors on different devices")
+        _one_device(x, y, norm_scale, gate, mod_scale, mod_shift)
         return _ResidualNorm.apply(x, y, norm_scale, gate, mod_scale, mod_shift, eps)
     lead = x.shape[:-2] if x.dim() >= 3 else ()
 

@@ -67,6 +67,35 @@ def _ptr(t: torch.Tensor | None) -> C.c_void_p:
     return C.c_void_p(0 if t is None else t.data_ptr())
 
 
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _launch(dev: torch.device, fn, what: str, *args) -> None:
+    """``fn(*args, stream)`` on ``dev``'s current stream; pointers may be plain integers.  The device is only
+    switched when it is not the current one: small calls are bound by what the host does for them."""
+    i = dev.index
+    if _current_device() == i:
+        rc = fn(*args, _raw_stream(i))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(i))
+    if rc:
+        _lib.check(rc, what)
+
+
+def _one_device(*tensors: torch.Tensor | None) -> torch.device:
+    """:func:`_need_cuda` for callers whose first tensor is never None."""
+    dev = tensors[0].device
+    if dev.type == "cuda":
+        for t in tensors:
+            if t is not None and t.device != dev:
+                break
+        else:
+            return dev
+    return _need_cuda(*tensors)
+
+
 def _rows2d(t: torch.Tensor) -> torch.Tensor:
     """View as [rows, last] with unit inner stride (copies only if it has to)."""
     t2 = t.reshape(-1, t.shape[-1])
@@ -248,13 +277,26 @@ def norm_mod_quant(x: torch.Tensor, norm_scale: torch.Tensor, mod_scale: torch.T
 
 
 def _mod_vec(name: str, what: str, t: torch.Tensor | None, nb: int, k: int) -> torch.Tensor | None:
-    """A per-sample vector [B, 1, K] / [B, K] as contiguous [B, K] with a 16-byte aligned base."""
+    """A per-sample vector [B, 1, K] / [B, K] as contiguous [B, K] values with a 16-byte aligned base."""
     if t is None:
         return None
     if t.dtype != torch.bfloat16 or t.numel() != nb * k or t.shape[-1] != k:
         raise ValueError(f"{name}: {what} must be bf16 with {nb} x {k} elements")
-    t = t.reshape(nb, k).contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _row_operand(t: torch.Tensor, k: int):
+    """(tensor to keep, address, leading dimension) of [..., K] rows as a kernel reads them."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, t.data_ptr(), k
+    t2 = _aligned_rows(t)
+    return t2, t2.data_ptr(), _row_stride(t2)
+
+
+def _opt_ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
@@ -269,11 +311,6 @@ def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
 def _row_stride(t2: torch.Tensor) -> int:
     """Leading dimension of a [rows, K] matrix (a single row may carry any stride)."""
     return t2.stride(0) if t2.shape[0] > 1 else t2.shape[1]
-
-
-def _span(t: torch.Tensor):
-    """First and last byte of a row matrix."""
-    return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * _row_stride(t) + t.shape[1]) * t.element_size()
 
 
 def _check_residual(name, x, y, norm_scale, k):
@@ -298,39 +335,39 @@ def residual_norm_quant(x: torch.Tensor, y: torch.Tensor, norm_scale: torch.Tens
     it may be x or y itself (in place).  Everything between loads and stores is fp32: the codes differ
     in rounding from ``norm_mod_quant(gate_residual(...))``, which rounds to bf16 after every step."""
     name = "residual_norm_quant"
-    dev = _need_cuda(x, y, norm_scale, gate, mod_scale, mod_shift, out)
+    dev = _one_device(x, y, norm_scale, gate, mod_scale, mod_shift, out)
     k = x.shape[-1]
     _check_residual(name, x, y, norm_scale, k)
     if k % HAD_BLOCK or k > 16384 or k == 0:
         raise ValueError(f"{name}: K={k} must be a multiple of {HAD_BLOCK} up to 16384")
     m = x.numel() // k
-    xq = torch.empty(m, k, dtype=torch.int8, device=dev)
+    xq = torch.empty((m, k), dtype=torch.int8, device=dev)
     sx = torch.empty(m, dtype=torch.float32, device=dev)
     if out is not None and (out.dtype != torch.bfloat16 or out.shape != x.shape):
         raise ValueError(f"{name}: out must be a bf16 tensor of x's shape")
     if m == 0:
         return (torch.empty_like(x) if out is None else out), xq, sx
     rows = x.shape[-2] if x.dim() >= 3 else m
-    x2, y2 = _aligned_rows(x), _aligned_rows(y)
+    x2, xp, ldx = _row_operand(x, k)
+    y2, yp, ldy = _row_operand(y, k)
     if out is None:
-        o2 = torch.empty(m, k, dtype=torch.bfloat16, device=dev)
-        out = o2.view(x.shape)
+        out = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+        op, ldo = out.data_ptr(), k
     else:
         o2 = _out_rows(name, out, k)
-        for what, src in (("x", x2), ("y", y2)):
-            (a0, a1), (b0, b1) = _span(o2), _span(src)
-            if a0 < b1 and b0 < a1 and not (a0 == b0 and _row_stride(o2) == _row_stride(src)):
+        op, ldo = o2.data_ptr(), _row_stride(o2)
+        for what, p, ld in (("x", xp, ldx), ("y", yp, ldy)):
+            if op < p + ((m - 1) * ld + k) * 2 and p < op + ((m - 1) * ldo + k) * 2 and not (op == p and ldo == ld):
                 raise ValueError(f"{name}: out overlaps {what} without being {what}")
         note_raw_write()
     if norm_scale.data_ptr() % 16:
         norm_scale = norm_scale.clone()
-    g, sc, sh = (_mod_vec(name, w, t, m // rows, k) for w, t in (("gate", gate), ("mod_scale", mod_scale),
-                                                                 ("mod_shift", mod_shift)))
-    with torch.cuda.device(dev):
-        rc = _lib.load().k2q_residual_norm_quant(
-            _ptr(x2), _row_stride(x2), _ptr(y2), _row_stride(y2), _ptr(g), _ptr(norm_scale), _ptr(sc), _ptr(sh), rows, m, k,
-            float(eps), _ptr(o2), _row_stride(o2), _ptr(xq), _ptr(sx), _stream(dev))
-    _lib.check(rc, "k2q_residual_norm_quant")
+    nb = m // rows
+    g = _mod_vec(name, "gate", gate, nb, k)
+    sc = _mod_vec(name, "mod_scale", mod_scale, nb, k)
+    sh = _mod_vec(name, "mod_shift", mod_shift, nb, k)
+    _launch(dev, _lib.load().k2q_residual_norm_quant, "k2q_residual_norm_quant", xp, ldx, yp, ldy, _opt_ptr(g),
+            norm_scale.data_ptr(), _opt_ptr(sc), _opt_ptr(sh), rows, m, k, eps, op, ldo, xq.data_ptr(), sx.data_ptr())
     return out, xq, sx
 
 
@@ -527,22 +564,20 @@ def gemv_w4a8(xq, sx, wq4, sw4, bias=None, u=None, bm=None, lora_scale: float = 
     """:func:`gemm_w4a8` for up to ``GEMV_ROWS`` token rows (one timestep vector per image, a short prompt): the
     same operands and the same bits, from a kernel that is bound by reading the 4-bit codes once."""
     name = "gemv_w4a8"
-    dev = _need_cuda(xq, sx, wq4, sw4, bias, u, bm)
+    dev = _one_device(xq, sx, wq4, sw4, bias, u, bm)
     m, n, k = _check_w4a8(name, xq, sx, wq4, sw4, bias, u, bm)
     if m > GEMV_ROWS:
         raise ValueError(f"{name}: {m} token rows; it takes up to {GEMV_ROWS} (gemm_w4a8 takes any number)")
     if out is not None:
         _check_out(name, out, m, n, dev)
-    y = out if out is not None else torch.empty(m, n, dtype=torch.bfloat16, device=dev)
+    y = out if out is not None else torch.empty((m, n), dtype=torch.bfloat16, device=dev)
     if m == 0:
         return y
     if sw4.data_ptr() % 16:
         sw4 = sw4.clone()
     ep = _epilogue(sx, bias, u, bm, lora_scale, act)
-    with torch.cuda.device(dev):
-        rc = _lib.load().k2q_gemv_w4a8(_ptr(xq), _ptr(wq4), _ptr(sw4), m, n, k, C.byref(ep), _ptr(y),
-                                       y.stride(0) if m > 1 else n, _stream(dev))
-    _lib.check(rc, "k2q_gemv_w4a8")
+    _launch(dev, _lib.load().k2q_gemv_w4a8, "k2q_gemv_w4a8", xq.data_ptr(), wq4.data_ptr(), sw4.data_ptr(), m, n, k, C.byref(ep),
+            y.data_ptr(), y.stride(0) if m > 1 else n)
     return y
 
 
@@ -704,7 +739,7 @@ class MatrixLayout:
 
 
 def _check_flat(name: str, layout: MatrixLayout, **tensors) -> torch.device:
-    dev = _need_cuda(*tensors.values(), layout.table)
+    dev = _one_device(*tensors.values(), layout.table)
     for what, t in tensors.items():
         if t.dtype != torch.float32 or t.numel() != layout.numel or not t.is_contiguous():
             raise ValueError(f"{name}: {what} must be a contiguous fp32 buffer of {layout.numel} elements")
@@ -741,12 +776,9 @@ def orthogonal_step_(param: torch.Tensor, grad: torch.Tensor, moment: torch.Tens
         raise ValueError(f"{name}: normsq must be one fp32 value on the buffers' device")
     pl = layout.plan
     ws = torch.empty(pl.workspace_bytes // 4, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        rc = _lib.load().k2q_orthogonal_step(
-            _ptr(param), _ptr(grad), _ptr(moment), C.byref(pl), _ptr(layout.table), float(lr), float(momentum), int(bool(nesterov)),
-            float(weight_decay), _STEP_SCALES[scale], int(steps), float(eps), float(max_norm), _ptr(normsq),
-            int(bool(zero_grad)), _ptr(ws), ws.numel() * 4, _stream(dev))
-    _lib.check(rc, "k2q_orthogonal_step")
+    _launch(dev, _lib.load().k2q_orthogonal_step, "k2q_orthogonal_step", param.data_ptr(), grad.data_ptr(), moment.data_ptr(),
+            C.byref(pl), layout.table.data_ptr(), lr, momentum, bool(nesterov), weight_decay, _STEP_SCALES[scale], int(steps), eps,
+            max_norm, _opt_ptr(normsq), bool(zero_grad), ws.data_ptr(), pl.workspace_bytes)
     note_raw_write()
 
 
@@ -762,10 +794,8 @@ def orthogonalize(u: torch.Tensor, layout: MatrixLayout, steps: int = 5, eps: fl
         raise ValueError(f"{name}: out overlaps u without being u")
     pl = layout.plan
     ws = torch.empty(pl.workspace_bytes // 4, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        rc = _lib.load().k2q_orthogonalize(_ptr(u), _ptr(out), C.byref(pl), _ptr(layout.table), int(steps), float(eps), _ptr(ws),
-                                           ws.numel() * 4, _stream(dev))
-    _lib.check(rc, "k2q_orthogonalize")
+    _launch(dev, _lib.load().k2q_orthogonalize, "k2q_orthogonalize", u.data_ptr(), out.data_ptr(), C.byref(pl),
+            layout.table.data_ptr(), int(steps), eps, ws.data_ptr(), pl.workspace_bytes)
     note_raw_write()
     return out
 
