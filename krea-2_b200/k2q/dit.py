@@ -226,6 +226,10 @@ class SimpleModulation(nn.Module):
 
 
 class SingleStreamBlock(nn.Module):
+    # set by ``modules.fuse_residual_norms``: the update of the stream behind the attention and the norm in front of
+    # the MLP run as one step (``ops.residual_norm_quant`` / ``fused.residual_norm``)
+    residual_fused = False
+
     def __init__(self, features, heads, multiplier, bias=False, kvheads=None):
         super().__init__()
         self.mod = DoubleSharedModulation(features)
@@ -242,14 +246,24 @@ class SingleStreamBlock(nn.Module):
             # quantisation passes (one read of the residual stream gives the codes of four Linears)
             lead = x.shape[:2]
             xq, sx = ops.norm_mod_quant(x, self.prenorm.scale.float(), prescale, preshift, self.prenorm.eps)
+            if self.residual_fused:
+                x, xq, sx = ops.residual_norm_quant(x, a.forward_codes(xq, sx, lead, rope, mask), self.postnorm.scale.float(),
+                                                    pregate, postscale, postshift, self.postnorm.eps)
+                return fused.gate_residual(x, postgate, m.forward_codes(xq, sx, lead))
             x = fused.gate_residual(x, pregate, a.forward_codes(xq, sx, lead, rope, mask))
             xq, sx = ops.norm_mod_quant(x, self.postnorm.scale.float(), postscale, postshift, self.postnorm.eps)
             return fused.gate_residual(x, postgate, m.forward_codes(xq, sx, lead))
+        if self.residual_fused:
+            x, h = fused.residual_norm(x, a(fused.norm_modulate(x, self.prenorm, prescale, preshift), rope, mask),
+                                       self.postnorm.scale.float(), pregate, postscale, postshift, self.postnorm.eps)
+            return fused.gate_residual(x, postgate, m(h))
         x = fused.gate_residual(x, pregate, a(fused.norm_modulate(x, self.prenorm, prescale, preshift), rope, mask))
         return fused.gate_residual(x, postgate, m(fused.norm_modulate(x, self.postnorm, postscale, postshift)))
 
 
 class TextFusionBlock(nn.Module):
+    residual_fused = False                       # see SingleStreamBlock
+
     def __init__(self, features, heads, multiplier, bias=False, kvheads=None):
         super().__init__()
         self.prenorm, self.postnorm = RMSNorm(features), RMSNorm(features)
@@ -257,6 +271,10 @@ class TextFusionBlock(nn.Module):
         self.mlp = SwiGLU(features, multiplier, bias)
 
     def forward(self, x, mask=None):
+        if self.residual_fused:
+            x, h = fused.residual_norm(x, self.attn(fused.norm_modulate(x, self.prenorm), None, mask), self.postnorm.scale.float(),
+                                       eps=self.postnorm.eps)
+            return x + self.mlp(h)
         x = x + self.attn(fused.norm_modulate(x, self.prenorm), None, mask)
         return x + self.mlp(fused.norm_modulate(x, self.postnorm))
 

@@ -476,6 +476,35 @@ def quantize_dit_convrot(dit, bits: int = 8, group: int = GROUP, had_block: int 
     return len(targets)
 
 
+def fuse_residual_norms(dit, fused: bool = True) -> int:
+    """Makes the blocks of a :class:`~k2q.dit.SingleStreamDiT` (its text-fusion blocks too) run the stream's update
+    behind the attention and the norm in front of the MLP as one step, in training and in sampling
+    (``fused.residual_norm``, ``ops.residual_norm_quant``).  That step is fp32 inside where the single kernels
+    round to bf16 after every operation as the reference's eager code does, so results differ in
+    their last bits; ``fused=False`` goes back.  Returns the number of blocks switched."""
+    n = 0
+    for block in dit.modules():
+        if hasattr(type(block), "residual_fused"):
+            block.residual_fused = bool(fused)
+            n += 1
+    return n
+
+
+def quantize_time_path(dit, bits: int = 4, group: int = GROUP, had_block: int = HAD_BLOCK) -> int:
+    """Replaces the Linears of the timestep MLP and of the modulation projection (``tmlp``, ``tproj``, mmdit.py:360-375), which
+    :func:`quantize_dit_convrot` leaves in bf16, with :class:`ConvRotLinear`; returns how many were replaced.  They
+    see one row per image: with ``bits=4`` such a product is one reading of the 4-bit codes (``ops.gemv_w4a8``),
+    a quarter of the bf16 weights' bytes in memory and per step.  The path is frozen (no backward copy); sampling and
+    adapter training both run through it."""
+    n = 0
+    for seq in (dit.tmlp, dit.tproj):
+        for name, child in list(seq.named_children()):
+            if isinstance(child, nn.Linear):
+                setattr(seq, name, ConvRotLinear(child, bits=bits, group=group, had_block=had_block, backward_copy=False))
+                n += 1
+    return n
+
+
 @torch.no_grad()
 def convrot_mlp_gelu(x: torch.Tensor, fc1: ConvRotLinear, fc2: ConvRotLinear) -> torch.Tensor:
     """Forward of ``Sequential(Linear, GELU(approximate="tanh"), Linear)`` (the shape of the DiT's

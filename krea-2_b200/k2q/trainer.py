@@ -3,6 +3,8 @@
 * :class:`FusedAdapterStep`  ``clip_grad_norm_`` + ``AdamW.step`` + ``zero_grad`` of all adapter
   parameters as two kernel launches over flat buffers (the reference runs them as a few thousand
   small launches over 516 tensors).
+* :class:`FusedOrthogonalStep`  the same place in the loop with an orthogonalised (Muon) update of every
+  adapter matrix instead of AdamW's, over the same flat buffers.
 * :func:`enable_prefetching_block_swap`  block swap whose frozen blocks live in pinned host memory:
   the next swapped block is copied in on a side stream while the current one computes, and paging a
   block out is free -- its codes never change, so the device copy is simply dropped.
@@ -19,24 +21,18 @@ from . import _lib, ops
 from .parallel import AdapterGradBuckets
 
 
-class FusedAdapterStep:
-    """AdamW (torch.optim.AdamW's update rule, decoupled weight decay) with global-norm gradient
-    clipping over the parameters of an :class:`~k2q.parallel.AdapterGradBuckets`.
+class _FlatAdapterStep:
+    """What the fused optimizer steps share: the parameters of an
+    :class:`~k2q.parallel.AdapterGradBuckets` as one flat fp32 buffer in the buckets' order (every
+    parameter's ``.data`` is re-pointed at its slice, values kept, so modules, ``state_dict`` and
+    ``save_lora`` (lora.py:154-172) see ordinary tensors), and the global gradient norm."""
 
-    Parameters, gradients and both moments are flat fp32 buffers in the buckets' order; every
-    parameter's ``.data`` is re-pointed at its slice (values kept), so modules, ``state_dict`` and
-    ``save_lora`` (lora.py:154-172) see ordinary tensors.  ``step()`` = ``buckets.finish()`` (the
-    exchange) -> gradient norm -> update -> gradients zeroed; call ``buckets.zero()`` is not needed
-    afterwards, the arrival counters are re-armed here.
-    """
-
-    def __init__(self, buckets: AdapterGradBuckets, lr: float = 1e-4, betas=(0.9, 0.999), eps: float = 1e-8,
-                 weight_decay: float = 0.01, max_grad_norm: float = 1.0):
+    def __init__(self, buckets: AdapterGradBuckets, lr: float, weight_decay: float, max_grad_norm: float):
         self.buckets = buckets
-        self.lr, self.betas, self.eps, self.weight_decay, self.max_grad_norm = lr, betas, eps, weight_decay, max_grad_norm
+        self.lr, self.weight_decay, self.max_grad_norm = lr, weight_decay, max_grad_norm
         g = buckets.flat
         if not g.is_cuda:
-            raise RuntimeError("FusedAdapterStep runs on CUDA tensors only; there is no CPU fallback")
+            raise RuntimeError(f"{type(self).__name__} runs on CUDA tensors only; there is no CPU fallback")
         self.param = torch.empty_like(g)
         off = 0
         for b in buckets.buckets:
@@ -46,7 +42,6 @@ class FusedAdapterStep:
                 p.data = self.param[off:off + n].view_as(p)
                 off += n
         self.m = torch.zeros_like(g)
-        self.v = torch.zeros_like(g)
         self.normsq = torch.zeros(1, dtype=torch.float32, device=g.device)
         self.ws = torch.empty(int(_lib.load().k2q_sumsq_workspace_bytes()) // 4, dtype=torch.float32, device=g.device)
         self.step_count = 0
@@ -55,29 +50,53 @@ class FusedAdapterStep:
         """Global L2 norm of the last clipped step's gradients (device scalar, no synchronisation)."""
         return self.normsq.sqrt()
 
+    def _clipping(self) -> bool:
+        """Leaves the gradients' sum of squares in ``normsq`` when the step clips."""
+        if not (self.max_grad_norm and self.max_grad_norm > 0):
+            return False
+        g = self.buckets.flat
+        with torch.cuda.device(g.device):
+            stream = C.c_void_p(torch.cuda.current_stream(g.device).cuda_stream)
+            _lib.check(_lib.load().k2q_sumsq_f32(C.c_void_p(g.data_ptr()), g.numel(), C.c_void_p(self.normsq.data_ptr()), 0,
+                                                 C.c_void_p(self.ws.data_ptr()), self.ws.numel() * 4, stream), "k2q_sumsq_f32")
+        return True
+
+    def _rearm(self) -> None:
+        for b in self.buckets.buckets:             # gradients are zero again: re-arm the arrival counters
+            b["pending"], b["launched"] = len(b["params"]), False
+
+
+class FusedAdapterStep(_FlatAdapterStep):
+    """AdamW (torch.optim.AdamW's update rule, decoupled weight decay) with global-norm gradient
+    clipping over the parameters of an :class:`~k2q.parallel.AdapterGradBuckets`.
+
+    Parameters, gradients and both moments are flat fp32 buffers.  ``step()`` = ``buckets.finish()`` (the
+    exchange) -> gradient norm -> update -> gradients zeroed; call ``buckets.zero()`` is not needed
+    afterwards, the arrival counters are re-armed here.
+    """
+
+    def __init__(self, buckets: AdapterGradBuckets, lr: float = 1e-4, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 0.01, max_grad_norm: float = 1.0):
+        super().__init__(buckets, lr, weight_decay, max_grad_norm)
+        self.betas, self.eps = betas, eps
+        self.v = torch.zeros_like(buckets.flat)
+
     @torch.no_grad()
     def step(self, lr: float | None = None) -> None:
         bk = self.buckets
         bk.finish()
         g = bk.flat
         dev = g.device
-        lib = _lib.load()
-        stream = C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
         self.step_count += 1
+        norm_ptr = C.c_void_p(self.normsq.data_ptr()) if self._clipping() else C.c_void_p(0)
         with torch.cuda.device(dev):
-            norm_ptr = C.c_void_p(0)
-            if self.max_grad_norm and self.max_grad_norm > 0:
-                _lib.check(lib.k2q_sumsq_f32(C.c_void_p(g.data_ptr()), g.numel(), C.c_void_p(self.normsq.data_ptr()), 0,
-                                             C.c_void_p(self.ws.data_ptr()), self.ws.numel() * 4, stream), "k2q_sumsq_f32")
-                norm_ptr = C.c_void_p(self.normsq.data_ptr())
-            _lib.check(lib.k2q_adamw_clip_f32(C.c_void_p(self.param.data_ptr()), C.c_void_p(g.data_ptr()),
-                                              C.c_void_p(self.m.data_ptr()), C.c_void_p(self.v.data_ptr()), g.numel(),
-                                              float(self.lr if lr is None else lr), float(self.betas[0]),
-                                              float(self.betas[1]), float(self.eps), float(self.weight_decay),
-                                              self.step_count, float(self.max_grad_norm or 0.0), norm_ptr, 1, stream),
-                       "k2q_adamw_clip_f32")
-        for b in bk.buckets:                       # gradients are zero again: re-arm the arrival counters
-            b["pending"], b["launched"] = len(b["params"]), False
+            stream = C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+            _lib.check(_lib.load().k2q_adamw_clip_f32(
+                C.c_void_p(self.param.data_ptr()), C.c_void_p(g.data_ptr()), C.c_void_p(self.m.data_ptr()),
+                C.c_void_p(self.v.data_ptr()), g.numel(), float(self.lr if lr is None else lr), float(self.betas[0]),
+                float(self.betas[1]), float(self.eps), float(self.weight_decay), self.step_count,
+                float(self.max_grad_norm or 0.0), norm_ptr, 1, stream), "k2q_adamw_clip_f32")
+        self._rearm()
 
     def state_dict(self) -> dict:
         return {"step": self.step_count, "m": self.m, "v": self.v}
@@ -86,6 +105,41 @@ class FusedAdapterStep:
         self.step_count = int(sd["step"])
         self.m.copy_(sd["m"])
         self.v.copy_(sd["v"])
+
+
+class FusedOrthogonalStep(_FlatAdapterStep):
+    """Orthogonalised updates (Muon) of the adapter matrices of an :class:`~k2q.parallel.AdapterGradBuckets`, in
+    :class:`FusedAdapterStep`'s place: momentum, Newton-Schulz orthogonalisation on each matrix's rank, and
+    the decoupled parameter step (``ops.orthogonal_step_``), with the same global-norm clipping.  Every
+    parameter must be a matrix whose short side is at most 64.  ``scale="rms"`` gives updates of AdamW's usual
+    size, so learning rates carry over."""
+
+    def __init__(self, buckets: AdapterGradBuckets, lr: float = 1e-4, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.01, max_grad_norm: float = 1.0, scale: str = "rms", steps: int = 5, eps: float = 1e-7):
+        shapes = [tuple(p.shape) for b in buckets.buckets for p in b["params"]]
+        if any(len(s) != 2 for s in shapes):
+            raise ValueError("FusedOrthogonalStep: every parameter must be a matrix")
+        self.layout = ops.MatrixLayout(shapes, buckets.flat.device)
+        super().__init__(buckets, lr, weight_decay, max_grad_norm)
+        self.momentum, self.nesterov, self.scale, self.steps, self.eps = momentum, nesterov, scale, steps, eps
+
+    @torch.no_grad()
+    def step(self, lr: float | None = None) -> None:
+        self.buckets.finish()
+        self.step_count += 1
+        clip = self._clipping()
+        ops.orthogonal_step_(self.param, self.buckets.flat, self.m, self.layout, lr=self.lr if lr is None else lr,
+                             momentum=self.momentum, nesterov=self.nesterov, weight_decay=self.weight_decay, scale=self.scale,
+                             steps=self.steps, eps=self.eps, max_norm=float(self.max_grad_norm or 0.0),
+                             normsq=self.normsq if clip else None, zero_grad=True)
+        self._rearm()
+
+    def state_dict(self) -> dict:
+        return {"step": self.step_count, "m": self.m}
+
+    def load_state_dict(self, sd: dict) -> None:
+        self.step_count = int(sd["step"])
+        self.m.copy_(sd["m"])
 
 
 class _PrefetchSwap:
