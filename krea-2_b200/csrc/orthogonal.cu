@@ -290,6 +290,7 @@ __device__ __forceinline__ void gram_body(const StepParams& a, const Tile& tile,
     }
     __syncthreads();
   }
+  pdl_launch_dependents();                     // the next kernel's blocks may line up; they wait for this one's end
   // the shares of the positions, added in order
   if (works) {
 #pragma unroll
@@ -331,6 +332,7 @@ __device__ __forceinline__ void gram_body(const StepParams& a, const Tile& tile,
 
 __global__ void __launch_bounds__(kThreads, 3) gram_kernel(const StepParams a) {
   extern __shared__ __align__(16) float smem[];
+  pdl_wait();
   const Tile tile = a.tiles[blockIdx.x];
   const Mat t = a.mats[tile.mat];
   K2Q_BY_SHAPE(gram_body)
@@ -406,6 +408,7 @@ __global__ void __launch_bounds__(WARPS * 32) poly_kernel(const StepParams a) {
   constexpr int kPolyThreads = WARPS * 32;
   extern __shared__ __align__(16) double sh[];
   __shared__ double inv;
+  pdl_wait();
   const Mat t = a.mats[blockIdx.x];
   const int s4 = up4(t.s), s8 = up8(t.s), nt = s4 >> 2, pairs = pairs_of(t.s), pitch = pitch64(t.s), n = s8 * pitch;
   double *g = sh, *q = sh + n, *x = sh + 2 * n, *y = sh + 3 * n;
@@ -440,6 +443,7 @@ __global__ void __launch_bounds__(WARPS * 32) poly_kernel(const StepParams a) {
   const double f = inv;
   for (int e = threadIdx.x; e < n; e += kPolyThreads) g[e] *= f * f;
   __syncthreads();
+  pdl_launch_dependents();
   for (int it = 0; it < a.steps; ++it) {
     double* factor = it == 0 ? x : q;          // the first factor is the product so far
     poly_step<true>(factor, g, g, tiles, s8);
@@ -603,6 +607,7 @@ __device__ __forceinline__ void apply_body(const StepParams& a, const Tile& tile
 
 __global__ void __launch_bounds__(kThreads, 2) apply_kernel(const StepParams a) {
   extern __shared__ __align__(16) float smem[];
+  pdl_wait();
   const Tile tile = a.tiles[blockIdx.x];
   const Mat t = a.mats[tile.mat];
   K2Q_BY_SHAPE(apply_body)
@@ -669,10 +674,9 @@ int run_steps(const char* name, const k2q_matrices* pl, const void* table, StepP
                           "cudaFuncSetAttribute(apply)"))
     return rc;
   const unsigned tiles = static_cast<unsigned>(pl->tiles);
-  gram_kernel<<<tiles, kThreads, kGramSmem, s>>>(a);
-  poly<<<static_cast<unsigned>(pl->count), pl->max_short <= 32 ? 256 : 512, poly_smem, s>>>(a);
-  apply_kernel<<<tiles, kThreads, apply_smem, s>>>(a);
-  return check_cuda(cudaGetLastError(), name);
+  if (int rc = launch_overlapped(gram_kernel, tiles, kThreads, kGramSmem, s, 1, name, a)) return rc;
+  if (int rc = launch_overlapped(poly, static_cast<unsigned>(pl->count), pl->max_short <= 32 ? 256u : 512u, poly_smem, s, 1, name, a)) return rc;
+  return launch_overlapped(apply_kernel, tiles, kThreads, apply_smem, s, 1, name, a);
 }
 
 }  // namespace
