@@ -59,7 +59,7 @@ __device__ __forceinline__ void finish(const GemvParams& p, int m, int n, float 
 
 __device__ __forceinline__ void mma_s8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                              uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -176,19 +176,24 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) gemv_kernel(const GemvParam
       out = out == (RING - 1) * kEntry ? 0u : out + kEntry;
       int acc[GP][MT][CT][4];
 #pragma unroll
-      for (int h = 0; h < GP; ++h) {
+      for (int h = 0; h < GP; ++h)
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
           for (int c = 0; c < CT; ++c) acc[h][t][c][0] = acc[h][t][c][1] = acc[h][t][c][2] = acc[h][t][c][3] = 0;
+      // the groups side by side, so that neighbouring MMAs do not wait for one another
 #pragma unroll
-        for (int jj = 0; jj < 2; ++jj) {                       // 64 of the group's codes: two words of each lane
-          uint4 x[2 * MT];
+      for (int jj = 0; jj < 2; ++jj) {                         // 64 of a group's codes: two words of each lane
+        uint4 x[GP][2 * MT];
+#pragma unroll
+        for (int h = 0; h < GP; ++h)
 #pragma unroll
           for (int t = 0; t < 2 * MT; ++t)
-            x[t] = t < MH ? *reinterpret_cast<const uint4*>(xg + h * 128 + xoff[t < MH ? t : 0] + jj * 16) : make_uint4(0, 0, 0, 0);
+            x[h][t] = t < MH ? *reinterpret_cast<const uint4*>(xg + h * 128 + xoff[t < MH ? t : 0] + jj * 16) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int h = 0; h < GP; ++h) {
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
               const uint4 v = wv[h][c];
@@ -196,8 +201,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) gemv_kernel(const GemvParam
               const uint32_t b0 = (word << 4) & 0xF0F0F0F0u, b1 = word & 0xF0F0F0F0u;
 #pragma unroll
               for (int t = 0; t < MT; ++t)
-                mma_s8_16832(acc[h][t][c], j ? x[2 * t].z : x[2 * t].x, j ? x[2 * t + 1].z : x[2 * t + 1].x,
-                             j ? x[2 * t].w : x[2 * t].y, j ? x[2 * t + 1].w : x[2 * t + 1].y, b0, b1);
+                mma_s8_16832(acc[h][t][c], j ? x[h][2 * t].z : x[h][2 * t].x, j ? x[h][2 * t + 1].z : x[h][2 * t + 1].x,
+                             j ? x[h][2 * t].w : x[h][2 * t].y, j ? x[h][2 * t + 1].w : x[h][2 * t + 1].y, b0, b1);
             }
           }
         }
