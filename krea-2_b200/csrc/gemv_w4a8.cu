@@ -33,6 +33,7 @@ struct GemvParams {
   int64_t ldu, ldb; int rank; float lora_scale; int act;
   __nv_bfloat16* y; int64_t ldy;
   int warps;                          // warps per CTA that multiply
+  int ks;                             // warps that share eight channels (ring kernel; `warps` then counts teams)
   int chunk;                          // groups of the tokens staged at a time
 };
 
@@ -76,6 +77,9 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
 }
 
 constexpr int kMaxWarps = 16;
+// named barriers (0 is __syncthreads)
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 constexpr int kSmemMax = 232448;
 
 // Groups [g0, g0 + chunk) of every token into shared memory, the even and the odd bytes of every eight apart.  A
@@ -97,6 +101,50 @@ __device__ __forceinline__ void deal_tokens(const GemvParams& p, uint8_t* xs, in
     const uint4 v = *at;
     *at = make_uint4(pick(v.x, v.y, 0x6420u), pick(v.x, v.y, 0x7531u), pick(v.z, v.w, 0x6420u), pick(v.z, v.w, 0x7531u));
     for (c += blockDim.x; c >= n; c -= n) ++m;
+  }
+}
+
+// 16 times the sums of GP groups: entry = this lane's codes, xg = the tokens at the first group, acc[h][t][c][0..1] token
+// 16 t + r, channels 8 c + 2 q, + 1, acc[..][2..3] token 16 t + r + 8.
+template <int MH, int CT, int GP>
+__device__ __forceinline__ void group_sums(uint32_t entry, const uint8_t* xg, const int (&xoff)[MH], int (&acc)[GP][(MH + 1) / 2][CT][4]) {
+  constexpr int MT = (MH + 1) / 2;
+  uint4 wv[GP][CT];
+#pragma unroll
+  for (int h = 0; h < GP; ++h)
+#pragma unroll
+    for (int c = 0; c < CT; ++c) wv[h][c] = lds16(entry + (h * CT + c) * 512);
+#pragma unroll
+  for (int h = 0; h < GP; ++h)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int c = 0; c < CT; ++c) acc[h][t][c][0] = acc[h][t][c][1] = acc[h][t][c][2] = acc[h][t][c][3] = 0;
+  // the groups side by side, so that neighbouring MMAs do not wait for one another
+#pragma unroll
+  for (int jj = 0; jj < 2; ++jj) {                         // 64 of a group's codes: two words of each lane
+    uint4 x[GP][2 * MT];
+#pragma unroll
+    for (int h = 0; h < GP; ++h)
+#pragma unroll
+      for (int t = 0; t < 2 * MT; ++t)
+        x[h][t] = t < MH ? *reinterpret_cast<const uint4*>(xg + h * 128 + xoff[t < MH ? t : 0] + jj * 16) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int h = 0; h < GP; ++h) {
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          const uint4 v = wv[h][c];
+          const uint32_t word = jj ? (j ? v.w : v.z) : (j ? v.y : v.x);
+          const uint32_t b0 = (word << 4) & 0xF0F0F0F0u, b1 = word & 0xF0F0F0F0u;
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+            mma_s8_16832(acc[h][t][c], j ? x[h][2 * t].z : x[h][2 * t].x, j ? x[h][2 * t + 1].z : x[h][2 * t + 1].x,
+                         j ? x[h][2 * t].w : x[h][2 * t].y, j ? x[h][2 * t + 1].w : x[h][2 * t + 1].y, b0, b1);
+        }
+      }
+    }
   }
 }
 
@@ -168,45 +216,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) gemv_kernel(const GemvParam
     const uint8_t* xg = xs;
     for (int g = 0; g < n; g += GP, xg += GP * 128) {
       cp_async_wait<RING - 2>();
-      uint4 wv[GP][CT];
-#pragma unroll
-      for (int h = 0; h < GP; ++h)
-#pragma unroll
-        for (int c = 0; c < CT; ++c) wv[h][c] = lds16(ring + out + (h * CT + c) * 512);
-      out = out == (RING - 1) * kEntry ? 0u : out + kEntry;
       int acc[GP][MT][CT][4];
-#pragma unroll
-      for (int h = 0; h < GP; ++h)
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int c = 0; c < CT; ++c) acc[h][t][c][0] = acc[h][t][c][1] = acc[h][t][c][2] = acc[h][t][c][3] = 0;
-      // the groups side by side, so that neighbouring MMAs do not wait for one another
-#pragma unroll
-      for (int jj = 0; jj < 2; ++jj) {                         // 64 of a group's codes: two words of each lane
-        uint4 x[GP][2 * MT];
-#pragma unroll
-        for (int h = 0; h < GP; ++h)
-#pragma unroll
-          for (int t = 0; t < 2 * MT; ++t)
-            x[h][t] = t < MH ? *reinterpret_cast<const uint4*>(xg + h * 128 + xoff[t < MH ? t : 0] + jj * 16) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-          for (int h = 0; h < GP; ++h) {
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-              const uint4 v = wv[h][c];
-              const uint32_t word = jj ? (j ? v.w : v.z) : (j ? v.y : v.x);
-              const uint32_t b0 = (word << 4) & 0xF0F0F0F0u, b1 = word & 0xF0F0F0F0u;
-#pragma unroll
-              for (int t = 0; t < MT; ++t)
-                mma_s8_16832(acc[h][t][c], j ? x[h][2 * t].z : x[h][2 * t].x, j ? x[h][2 * t + 1].z : x[h][2 * t + 1].x,
-                             j ? x[h][2 * t].w : x[h][2 * t].y, j ? x[h][2 * t + 1].w : x[h][2 * t + 1].y, b0, b1);
-            }
-          }
-        }
-      }
+      group_sums<MH, CT, GP>(ring + out, xg, xoff, acc);
+      out = out == (RING - 1) * kEntry ? 0u : out + kEntry;
       request();
 #pragma unroll
       for (int h = 0; h < GP; ++h) {
@@ -242,6 +254,160 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) gemv_kernel(const GemvParam
       }
 }
 
+// Few channels per SM: p.ks warps share eight channels.  They take blocks of G groups in turn, keep a block's sums in
+// registers, and pass the running values on in block order: warp j folds its block when they arrive from warp j - 1, and
+// hands them to warp j + 1 (the last to the first, for the next round), through a slot in shared memory and a named
+// barrier of the two warps.  A block's arithmetic takes many times the fold, so that nobody waits in the steady state.  A
+// slot or barrier is used again only after the values have gone round once, hence after its reader.
+template <int MH, int RING>
+__global__ void __launch_bounds__(kMaxWarps * 32, 1) gemv_ring_kernel(const GemvParams p) {
+  constexpr int MT = (MH + 1) / 2, GP = 4, G = 8, IT = G / GP, V = MH == 1 ? 2 : 4;   // V values per lane and token tile
+  constexpr uint32_t kEntry = GP * 512;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
+  const int groups = p.K >> 7, blocks = (groups + G - 1) / G, ks = p.ks;
+  const int team = warp / ks, j = warp - team * ks, n0 = (blockIdx.x * p.warps + team) * 8;
+  const bool live = team < p.warps && n0 < p.N;                // the other warps only help to stage the tokens
+  // shared memory: rings | scales [channel][group] | slots | tokens
+  const uint32_t ring = smem_u32(smem) + warp * (RING * kEntry) + lane * 16;
+  uint8_t* scales = smem + p.warps * ks * RING * kEntry;
+  float* slots = reinterpret_cast<float*>(scales + p.warps * groups * 16);
+  uint8_t* xs = reinterpret_cast<uint8_t*>(slots + p.warps * ks * MT * V * 32);
+  pdl_wait();
+  request_tokens(p, smem_u32(xs), 0);
+  {
+    const int first = blockIdx.x * p.warps * 8, n = min(p.warps * 8, p.N - first) * groups / 8;
+    const __nv_bfloat16* s = p.sw + static_cast<int64_t>(first) * groups;     // one contiguous block
+    for (int c = threadIdx.x; c < n; c += blockDim.x) cp_async16(smem_u32(scales) + c * 16, s + c * 8, 16);
+  }
+  cp_async_commit();
+  const int64_t row_bytes = p.K >> 1;
+  const uint8_t* src = p.wq + (n0 + r) * row_bytes + static_cast<int64_t>(j) * G * 64 + q * 16;
+  int next = live ? j * G : groups;                            // group of the next request; past the end: nothing left
+  uint32_t in = 0, out = 0;
+  auto request = [&]() {
+#pragma unroll
+    for (int h = 0; h < GP; ++h)
+      if (next + h < groups) cp_async16(ring + in + h * 512, src + h * 64, 16);
+    next += GP;
+    src += GP * 64;
+    if ((next & (G - 1)) == 0) {                               // the warp's block is requested: on to its next one
+      next += (ks - 1) * G;
+      src += static_cast<int64_t>(ks - 1) * G * 64;
+    }
+    in = in == (RING - 1) * kEntry ? 0u : in + kEntry;
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < RING - 1; ++i) request();
+  cp_async_wait<RING - 1>();
+  deal_tokens(p, xs, 0);
+  __syncthreads();
+  int xoff[MH];                                                // this lane's place in the tokens
+#pragma unroll
+  for (int t = 0; t < MH; ++t) {
+    const int tok = t * 8 + r;                                 // rows past M: any row, the result is not kept
+    xoff[t] = (tok < p.M ? tok : p.M - 1) * (p.chunk * 128 + 16) + q * 32;
+  }
+  const __nv_bfloat16* sc = reinterpret_cast<const __nv_bfloat16*>(scales) + (team * 8 + 2 * q) * groups;
+  const int rounds = (blocks + ks - 1) / ks;
+  const int prev = j == 0 ? ks - 1 : j - 1;
+  float run[MT][V] = {};
+  int g0 = 0;                                                  // first group of the staged tokens
+  for (int rd = 0; rd < rounds; ++rd) {
+    if (rd * ks * G >= g0 + p.chunk) {                         // the chunk is a multiple of a round
+      g0 += p.chunk;
+      __syncthreads();
+      request_tokens(p, smem_u32(xs), g0);
+      cp_async_commit();
+      cp_async_wait<0>();
+      deal_tokens(p, xs, g0);
+      __syncthreads();
+    }
+    const int blk = rd * ks + j, b0 = blk * G;
+    if (!live || blk >= blocks) continue;
+    float sum[IT][GP][MT][V];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      cp_async_wait<RING - 2>();
+      int acc[GP][MT][1][4];
+      group_sums<MH, 1, GP>(ring + out, xs + (b0 + i * GP - g0) * 128, xoff, acc);
+      out = out == (RING - 1) * kEntry ? 0u : out + kEntry;
+      request();
+#pragma unroll
+      for (int h = 0; h < GP; ++h)
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int v = 0; v < V; ++v) sum[i][h][t][v] = static_cast<float>(acc[h][t][0][v]);
+    }
+    if (blk > 0) {
+      bar_sync(1 + team * ks + prev, 64);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int v = 0; v < V; ++v) run[t][v] = slots[((team * ks + prev) * MT * V + t * V + v) * 32 + lane];
+    }
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+      for (int h = 0; h < GP; ++h) {
+        const int g = b0 + i * GP + h;
+        if (g < groups) {
+          // the group sums hold 16 times the codes' product
+          const float s0 = __bfloat162float(sc[g]) * 0.0625f, s1 = __bfloat162float(sc[groups + g]) * 0.0625f;
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int v = 0; v < V; ++v) run[t][v] = fmaf(sum[i][h][t][v], (v & 1) ? s1 : s0, run[t][v]);
+        }
+      }
+    if (blk + 1 < blocks) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int v = 0; v < V; ++v) slots[(warp * MT * V + t * V + v) * 32 + lane] = run[t][v];
+      bar_arrive(1 + warp, 64);
+    } else {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int m = t * 16 + r + 8 * (v >> 1), n = n0 + 2 * q + (v & 1);
+          if (m < p.M) finish(p, m, n, run[t][v]);
+        }
+    }
+  }
+}
+
+// groups of the tokens that fit beside `ks` warps per team, in whole rounds
+template <int MH, int RING>
+int ring_chunk(const GemvParams& p, int teams, int ks, int* fixed) {
+  constexpr int MT = (MH + 1) / 2, G = 8, V = MH == 1 ? 2 : 4;
+  *fixed = teams * ks * (RING * 2048 + MT * V * 32 * 4) + teams * (p.K >> 7) * 16;
+  return *fixed >= kSmemMax ? 0 : ((kSmemMax - *fixed) / p.M - 16) / 128 / (G * ks) * (G * ks);
+}
+
+template <int MH, int RING>
+int launch_ring(GemvParams p, int teams, int ks, cudaStream_t stream) {
+  constexpr int G = 8;
+  const int groups = p.K >> 7, warps = teams * ks;
+  int fixed = 0;
+  const int chunk = ring_chunk<MH, RING>(p, teams, ks, &fixed);
+  const int all_groups = (groups + G * ks - 1) / (G * ks) * (G * ks);
+  p.chunk = chunk < all_groups ? chunk : all_groups;
+  p.warps = teams;
+  p.ks = ks;
+  const int smem = fixed + p.M * (p.chunk * 128 + 16);
+  auto kern = gemv_ring_kernel<MH, RING>;
+  if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                          "cudaFuncSetAttribute(gemv_w4a8)"))
+    return rc;
+  const int tiles = p.N / 8, all = warps > 8 ? warps : 8;      // eight warps at least stage the tokens
+  return launch_overlapped(kern, static_cast<unsigned>((tiles + teams - 1) / teams), static_cast<unsigned>(all * 32),
+                           static_cast<size_t>(smem), stream, 1, "gemv_w4a8 launch", p);
+}
+
 template <int MH, int CT, int GP, int RING>
 int launch_one(GemvParams p, int warps, cudaStream_t stream) {
   const int tiles = p.N / (8 * CT), groups = p.K >> 7;
@@ -271,6 +437,15 @@ int launch_gemv(const GemvParams& p, cudaStream_t stream) {
   if (warps > kMaxWarps) warps = kMaxWarps;
   const int room = 64 * 1024 / (groups * 16 * ct);             // the scales stay in shared memory
   if (warps > room) warps = room;
+  // few channels: the contraction is split among 15 warps at most (a named barrier each)
+  int ks = 15 / warps;
+  const int blocks = (groups + 7) / 8;
+  if (ks > blocks) ks = blocks;
+  if constexpr (MH <= 2) {
+    int fixed;
+    while (ks >= 2 && ring_chunk<MH, 4>(p, warps, ks, &fixed) == 0) --ks;
+    if (ct == 1 && ks >= 2) return launch_ring<MH, 4>(p, warps, ks, stream);
+  }
   if (ct == 2) return launch_one<MH, 2, 2, MH == 1 ? 4 : 3>(p, warps, stream);
   return warps <= 8 ? launch_one<MH, 1, 4, 6>(p, warps, stream) : launch_one<MH, 1, 4, 4>(p, warps, stream);
 }
