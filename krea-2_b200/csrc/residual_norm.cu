@@ -574,38 +574,40 @@ __global__ void __launch_bounds__(32 * kSumGroups) residual_sums_kernel(const Su
   __shared__ float s[kSumGroups][3][32];
   const int col = threadIdx.x & 31, grp = threadIdx.x >> 5;
   const int k = blockIdx.x * 32 + col;
-  const int64_t b = blockIdx.y;
   const bool ok = k < p.K;
   pdl_wait();
-  float a[3] = {0.f, 0.f, 0.f};
-  if (ok) {
+  for (int64_t b = blockIdx.y; b < p.B; b += gridDim.y) {
+    float a[3] = {0.f, 0.f, 0.f};
+    if (ok) {
 #pragma unroll 4
-    for (int c = grp; c < p.chunks; c += kSumGroups) {
-      const float* src = p.part + ((b * p.chunks + c) * 3) * p.K + k;
-      a[0] += src[0];
-      a[1] += src[p.K];
-      a[2] += src[2 * static_cast<int64_t>(p.K)];
+      for (int c = grp; c < p.chunks; c += kSumGroups) {
+        const float* src = p.part + ((b * p.chunks + c) * 3) * p.K + k;
+        a[0] += src[0];
+        a[1] += src[p.K];
+        a[2] += src[2 * static_cast<int64_t>(p.K)];
+      }
     }
-  }
 #pragma unroll
-  for (int j = 0; j < 3; ++j) s[grp][j][col] = a[j];
-  __syncthreads();
-  if (grp == 0 && ok) {
+    for (int j = 0; j < 3; ++j) s[grp][j][col] = a[j];
+    __syncthreads();
+    if (grp == 0 && ok) {
 #pragma unroll
-    for (int j = 0; j < 3; ++j) {
-      a[j] = s[0][j][col];
+      for (int j = 0; j < 3; ++j) {
+        a[j] = s[0][j][col];
 #pragma unroll
-      for (int g = 1; g < kSumGroups; ++g) a[j] += s[g][j][col];
+        for (int g = 1; g < kSumGroups; ++g) a[j] += s[g][j][col];
+      }
+      const int64_t at = b * p.K + k;
+      if (p.dgate != nullptr) p.dgate[at] = __float2bfloat16_rn(a[0]);
+      if (p.dmscale != nullptr) p.dmscale[at] = __float2bfloat16_rn(a[1] * (1.0f + p.normw[k]));
+      if (p.dmshift != nullptr) p.dmshift[at] = __float2bfloat16_rn(a[2]);
+      if (p.dnorm != nullptr) {
+        const float d = p.mscale != nullptr ? a[1] * (1.0f + __bfloat162float(p.mscale[at])) : a[1];
+        if (p.B == 1) p.dnorm[k] = d;
+        else p.share[at] = d;
+      }
     }
-    const int64_t at = b * p.K + k;
-    if (p.dgate != nullptr) p.dgate[at] = __float2bfloat16_rn(a[0]);
-    if (p.dmscale != nullptr) p.dmscale[at] = __float2bfloat16_rn(a[1] * (1.0f + p.normw[k]));
-    if (p.dmshift != nullptr) p.dmshift[at] = __float2bfloat16_rn(a[2]);
-    if (p.dnorm != nullptr) {
-      const float d = p.mscale != nullptr ? a[1] * (1.0f + __bfloat162float(p.mscale[at])) : a[1];
-      if (p.B == 1) p.dnorm[k] = d;
-      else p.share[at] = d;
-    }
+    __syncthreads();                           // the sums have been read before the next sample's are written
   }
 }
 
@@ -704,6 +706,7 @@ int k2q_residual_norm_quant(const void* x_bf16, int64_t ldx, const void* y_bf16,
   p.stream = static_cast<__nv_bfloat16*>(stream_bf16); p.lds = lds; p.xq = xq; p.sx = sx;
   if (int rc = check_common(name, p, K, 128)) return rc;
   if (M == 0) return K2Q_OK;
+  if (!p.gate && !p.mscale && !p.mshift) p.rows_per_batch = rows_per_batch = M;    // nothing tells the samples apart
   if (!p.x || !p.y || !p.stream || !xq || !sx) return fail(K2Q_EINVAL, "%s: NULL operand", name);
   if (bad_rows(p.x, ldx, K) || bad_rows(p.y, ldy, K) || bad_rows(p.stream, lds, K) || off16(xq))
     return fail(K2Q_EINVAL, "%s: rows must be 16-byte aligned with a leading dimension >= K", name);
@@ -736,6 +739,7 @@ int k2q_residual_norm_fwd(const void* x_bf16, int64_t ldx, const void* y_bf16, i
   p.h = static_cast<__nv_bfloat16*>(h_bf16); p.ldh = ldh; p.rstd = rstd;
   if (int rc = check_common(name, p, K, 8)) return rc;
   if (M == 0) return K2Q_OK;
+  if (!p.gate && !p.mscale && !p.mshift) p.rows_per_batch = rows_per_batch = M;    // nothing tells the samples apart
   if (!p.x || !p.y || !p.stream || !p.h || !rstd) return fail(K2Q_EINVAL, "%s: NULL operand", name);
   if (bad_rows(p.x, ldx, K) || bad_rows(p.y, ldy, K) || bad_rows(p.stream, lds, K) || bad_rows(p.h, ldh, K))
     return fail(K2Q_EINVAL, "%s: rows must be 16-byte aligned with a leading dimension >= K", name);
@@ -779,6 +783,7 @@ int k2q_residual_norm_bwd(const void* dstream_bf16, int64_t ldds, const void* dh
   if (bad_rows(p.stream, lds, K) || (p.dstream && bad_rows(p.dstream, ldds, K)) || (p.dh && bad_rows(p.dh, lddh, K)) ||
       (p.y && bad_rows(p.y, ldy, K)) || (p.dx && bad_rows(p.dx, lddx, K)) || (p.dy && bad_rows(p.dy, lddy, K)))
     return fail(K2Q_EINVAL, "%s: rows must be 16-byte aligned with a leading dimension >= K", name);
+  if (!p.gate && !p.mscale && !dmod_scale_bf16 && !dmod_shift_bf16) p.rows_per_batch = rows_per_batch = M;
   if (dgate_bf16 && (!p.gate || !p.y)) return fail(K2Q_EINVAL, "%s: the gate's gradient needs gate and y", name);
   const int64_t B = M / rows_per_batch;
   const bool sums = dgate_bf16 || dmod_scale_bf16 || dmod_shift_bf16 || dnorm;
@@ -791,7 +796,6 @@ int k2q_residual_norm_bwd(const void* dstream_bf16, int64_t ldds, const void* dh
     p.part = static_cast<float*>(ws);
   }
   if (B * p.chunks > 0x7fffffffLL) return fail(K2Q_EINVAL, "%s: too many samples (%lld)", name, (long long)B);
-  if (sums && (B > 65535)) return fail(K2Q_EINVAL, "%s: sums over the rows of more than 65535 samples", name);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (shape.smem > 0) {
     if (int rc = check_cuda(cudaFuncSetAttribute(kBwd[shape.slot], cudaFuncAttributeMaxDynamicSharedMemorySize, shape.smem),
@@ -808,7 +812,7 @@ int k2q_residual_norm_bwd(const void* dstream_bf16, int64_t ldds, const void* dh
   q.dmshift = static_cast<__nv_bfloat16*>(dmod_shift_bf16); q.dnorm = dnorm;
   q.share = p.part + B * p.chunks * 3 * static_cast<int64_t>(p.K);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.K + 31) / 32), static_cast<unsigned>(B));
+  cfg.gridDim = dim3(static_cast<unsigned>((p.K + 31) / 32), static_cast<unsigned>(B < 65535 ? B : 65535));
   cfg.blockDim = dim3(32 * kSumGroups);
   cfg.stream = s;
   cudaLaunchAttribute attr{};

@@ -246,15 +246,14 @@ class _ResidualNorm(torch.autograd.Function):
         g = _mod_vec("residual_norm", "gate", gate, nb, k)
         sc = _mod_vec("residual_norm", "mod_scale", mod_scale, nb, k)
         sh = _mod_vec("residual_norm", "mod_shift", mod_shift, nb, k)
-        stream = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
-        h = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+        stream = torch.empty_like(x, memory_format=torch.contiguous_format)
+        h = torch.empty_like(stream)
         rstd = torch.empty(m, dtype=torch.float32, device=dev)
         _launch(dev, _lib.load().k2q_residual_norm_fwd, "k2q_residual_norm_fwd", xp, ldx, yp, ldy, _opt_ptr(g), w.data_ptr(),
                 _opt_ptr(sc), _opt_ptr(sh), rows, m, k, eps, stream.data_ptr(), k, h.data_ptr(), k, rstd.data_ptr())
         ctx.save_for_backward(stream, rstd, w, g, sc, y2 if ctx.needs_input_grad[3] else None)
         ctx.dims = (rows, m, k)
-        ctx.shapes = (x.shape, norm_scale.shape, None if gate is None else gate.shape,
-                      None if mod_scale is None else mod_scale.shape, None if mod_shift is None else mod_shift.shape)
+        ctx.shift_shape = None if mod_shift is None else mod_shift.shape
         ctx.set_materialize_grads(False)
         return stream, h
 
@@ -265,24 +264,22 @@ class _ResidualNorm(torch.autograd.Function):
         if ds is None and dh is None:
             return (None,) * 7
         need_x, need_y, need_w, need_g, need_sc, need_sh, _ = ctx.needs_input_grad
-        xs, wshape, gs, scs, shs = ctx.shapes
         rows, m, k = ctx.dims
         dev = stream.device
 
         def grad_rows(t):
             return (None, 0, 0) if t is None else _row_operand(t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16), k)
 
-        def new(shape, wanted):
-            return torch.empty(shape, dtype=torch.bfloat16, device=dev) if wanted else None
-
         ds2, dsp, ldds = grad_rows(ds)
         dh2, dhp, lddh = grad_rows(dh)
         _, yp, ldy = (None, 0, 0) if y2 is None else _row_operand(y2, k)
         same = g is None                               # without a gate dy equals dx: one tensor serves both
-        dx = new(xs, need_x or (same and need_y))
-        dy = new(xs, need_y and not same)
-        dg, dsc, dsh = new(gs, need_g), new(scs, need_sc), new(shs, need_sh)
-        dw = torch.empty(wshape, dtype=torch.float32, device=dev) if need_w else None
+        dx = torch.empty_like(stream) if need_x or (same and need_y) else None
+        dy = torch.empty_like(stream) if need_y and not same else None
+        dg = torch.empty_like(g) if need_g else None
+        dsc = torch.empty_like(sc) if need_sc else None
+        dsh = torch.empty(ctx.shift_shape, dtype=torch.bfloat16, device=dev) if need_sh else None
+        dw = torch.empty_like(w) if need_w else None
         lib = _lib.load()
         ws, ws_bytes = None, 0
         if need_g or need_sc or need_sh or need_w:
@@ -307,7 +304,7 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, norm_scale: torch.Tensor, ga
             and _kernel_ok(x, y, gate, mod_scale, mod_shift)):
         _check_residual("residual_norm", x, y, norm_scale, k)
         _one_device(x, y, norm_scale, gate, mod_scale, mod_shift)
-        return _ResidualNorm.apply(x, y, norm_scale, gate, mod_scale, mod_shift, eps)
+        return _ResidualNorm.apply(x, y, norm_scale, gate, mod_scale, mod_shift, float(eps))
     lead = x.shape[:-2] if x.dim() >= 3 else ()
 
     def vec(t):

@@ -496,13 +496,15 @@ def quantize_time_path(dit, bits: int = 4, group: int = GROUP, had_block: int = 
     see one row per image: with ``bits=4`` such a product is one reading of the 4-bit codes (``ops.gemv_w4a8``),
     a quarter of the bf16 weights' bytes in memory and per step.  The path is frozen (no backward copy); sampling and
     adapter training both run through it."""
-    n = 0
-    for seq in (dit.tmlp, dit.tproj):
-        for name, child in list(seq.named_children()):
-            if isinstance(child, nn.Linear):
-                setattr(seq, name, ConvRotLinear(child, bits=bits, group=group, had_block=had_block, backward_copy=False))
-                n += 1
-    return n
+    targets = [(seq, name, child) for seq in (dit.tmlp, dit.tproj) for name, child in seq.named_children()
+               if isinstance(child, nn.Linear)]
+    for _, name, child in targets:             # all or none
+        if child.in_features % HAD_BLOCK or child.out_features % 16:
+            raise ValueError(f"time path: a Linear of {child.in_features} to {child.out_features} features cannot be rotated "
+                             f"in blocks of {HAD_BLOCK}")
+    for seq, name, child in targets:
+        setattr(seq, name, ConvRotLinear(child, bits=bits, group=group, had_block=had_block, backward_copy=False))
+    return len(targets)
 
 
 @torch.no_grad()

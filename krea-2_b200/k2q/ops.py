@@ -351,7 +351,7 @@ def residual_norm_quant(x: torch.Tensor, y: torch.Tensor, norm_scale: torch.Tens
     x2, xp, ldx = _row_operand(x, k)
     y2, yp, ldy = _row_operand(y, k)
     if out is None:
-        out = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
         op, ldo = out.data_ptr(), k
     else:
         o2 = _out_rows(name, out, k)
@@ -360,6 +360,8 @@ def residual_norm_quant(x: torch.Tensor, y: torch.Tensor, norm_scale: torch.Tens
             if op < p + ((m - 1) * ld + k) * 2 and p < op + ((m - 1) * ldo + k) * 2 and not (op == p and ldo == ld):
                 raise ValueError(f"{name}: out overlaps {what} without being {what}")
         note_raw_write()
+        if not out.is_inference():
+            torch.autograd.graph.increment_version(out)      # a graph that saved it must not read the new values
     if norm_scale.data_ptr() % 16:
         norm_scale = norm_scale.clone()
     nb = m // rows
@@ -367,7 +369,7 @@ def residual_norm_quant(x: torch.Tensor, y: torch.Tensor, norm_scale: torch.Tens
     sc = _mod_vec(name, "mod_scale", mod_scale, nb, k)
     sh = _mod_vec(name, "mod_shift", mod_shift, nb, k)
     _launch(dev, _lib.load().k2q_residual_norm_quant, "k2q_residual_norm_quant", xp, ldx, yp, ldy, _opt_ptr(g),
-            norm_scale.data_ptr(), _opt_ptr(sc), _opt_ptr(sh), rows, m, k, eps, op, ldo, xq.data_ptr(), sx.data_ptr())
+            norm_scale.data_ptr(), _opt_ptr(sc), _opt_ptr(sh), rows, m, k, float(eps), op, ldo, xq.data_ptr(), sx.data_ptr())
     return out, xq, sx
 
 
@@ -777,8 +779,8 @@ def orthogonal_step_(param: torch.Tensor, grad: torch.Tensor, moment: torch.Tens
     pl = layout.plan
     ws = torch.empty(pl.workspace_bytes // 4, dtype=torch.float32, device=dev)
     _launch(dev, _lib.load().k2q_orthogonal_step, "k2q_orthogonal_step", param.data_ptr(), grad.data_ptr(), moment.data_ptr(),
-            C.byref(pl), layout.table.data_ptr(), lr, momentum, bool(nesterov), weight_decay, _STEP_SCALES[scale], int(steps), eps,
-            max_norm, _opt_ptr(normsq), bool(zero_grad), ws.data_ptr(), pl.workspace_bytes)
+            C.byref(pl), layout.table.data_ptr(), float(lr), float(momentum), bool(nesterov), float(weight_decay),
+            _STEP_SCALES[scale], int(steps), float(eps), float(max_norm), _opt_ptr(normsq), bool(zero_grad), ws.data_ptr(), pl.workspace_bytes)
     note_raw_write()
 
 
@@ -795,7 +797,7 @@ def orthogonalize(u: torch.Tensor, layout: MatrixLayout, steps: int = 5, eps: fl
     pl = layout.plan
     ws = torch.empty(pl.workspace_bytes // 4, dtype=torch.float32, device=dev)
     _launch(dev, _lib.load().k2q_orthogonalize, "k2q_orthogonalize", u.data_ptr(), out.data_ptr(), C.byref(pl),
-            layout.table.data_ptr(), int(steps), eps, ws.data_ptr(), pl.workspace_bytes)
+            layout.table.data_ptr(), int(steps), float(eps), ws.data_ptr(), pl.workspace_bytes)
     note_raw_write()
     return out
 

@@ -126,6 +126,14 @@ def test_checkpointed_training_step_captures_nothing_stale():
     assert torch.equal(grads[0], grads[1])
 
 
+def test_time_path_is_quantised_whole_or_not_at_all():
+    from k2q import dit, modules
+    m = dit.SingleStreamDiT(dit.DiTConfig(**dict(CFG, features=192, heads=2, kvheads=2))).to(torch.bfloat16).cuda()
+    with pytest.raises(ValueError):
+        modules.quantize_time_path(m)
+    assert all(type(c) is not modules.ConvRotLinear for seq in (m.tmlp, m.tproj) for c in seq)
+
+
 def test_orthogonal_step_refuses_vectors_and_large_ranks():
     from k2q import parallel, trainer
     for shape in ((300,), (65, 70)):

@@ -258,6 +258,70 @@ def test_repeatable_on_side_stream_and_in_a_graph():
     assert all(torch.equal(u, v) for u, v in zip(*runs))
 
 
+@pytest.mark.gpu
+def test_rows_past_32_bits_and_many_samples():
+    """More than 2^31 elements: the last rows, alone, give the same; 70000 samples of one row, summed."""
+    m, k = 350000, 6144
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.empty(1, m, k, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    y = torch.empty_like(x).normal_(generator=g)
+    w = torch.randn(k, generator=g, device="cuda") * 0.1
+    gate, sc, sh = ((torch.randn(1, 1, k, generator=g, device="cuda") * 0.5).bfloat16() for _ in range(3))
+    stream, xq, sx = ops.residual_norm_quant(x, y, w, gate, sc, sh)
+    few = ops.residual_norm_quant(x[:, -7:].contiguous(), y[:, -7:].contiguous(), w, gate, sc, sh)
+    assert torch.equal(stream[:, -7:], few[0]) and torch.equal(xq[-7:], few[1]) and torch.equal(sx[-7:], few[2])
+    del stream, xq, sx
+    s, h = fused.residual_norm(x, y, w, gate, sc, sh)
+    s7, h7 = fused.residual_norm(x[:, -7:].contiguous(), y[:, -7:].contiguous(), w, gate, sc, sh)
+    assert torch.equal(s[:, -7:], s7) and torch.equal(h[:, -7:], h7)
+    del x, y, s, h
+    b, k = 70000, 16
+    x = torch.randn(b, 1, k, generator=g, device="cuda").bfloat16()
+    y = torch.randn(b, 1, k, generator=g, device="cuda").bfloat16()
+    gate = torch.randn(b, 1, k, generator=g, device="cuda").bfloat16().requires_grad_(True)
+    s, _ = fused.residual_norm(x, y, torch.zeros(k, device="cuda"), gate)
+    (gg,) = torch.autograd.grad(s, gate, x)
+    assert torch.equal(gg, (x.float() * y.float()).bfloat16())
+
+
+@pytest.mark.gpu
+def test_backward_captured_in_a_graph():
+    t = make(2, 40, 512, True, 71, "cuda")
+    names = ("x", "y", "w", "gate", "sc", "sh")
+
+    def step(leaf):
+        out = fused.residual_norm(*(leaf[n] for n in names))
+        return torch.autograd.grad(out, [leaf[n] for n in names], (t["ds"], t["dh"]))
+
+    eager = {n: t[n].clone().requires_grad_(True) for n in names}
+    want = step(eager)
+    leaf = {n: t[n].clone().requires_grad_(True) for n in names}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(leaf)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = step(leaf)
+    for g in got:
+        g.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_in_place_write_is_seen_by_autograd():
+    t = make(1, 4, 256, False, 81, "cuda")
+    x = t["x"].clone().requires_grad_(True)
+    stream, h = fused.residual_norm(x, t["y"], t["w"])
+    kept = stream.detach()
+    ops.residual_norm_quant(t["x"], t["y"], t["w"], out=kept)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(h, x, t["dh"])
+
+
 # ---------------------------------------------------------------------------------------------- no GPU
 @pytest.mark.parametrize("modulated", [False, True])
 def test_composed_form_on_cpu(modulated):
