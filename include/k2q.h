@@ -352,7 +352,7 @@ int k2q_adamw_clip_f32(float* p, float* g, float* m, float* v, int64_t n, float 
 typedef struct k2q_matrices {
   int64_t count, total;                  /* matrices; elements of a flat buffer            */
   int64_t table_bytes, workspace_bytes;
-  int64_t piece, tiles;                  /* columns per piece of a long side; pieces       */
+  int64_t piece, tiles;                  /* sub-blocks per thread block; thread blocks       */
   int32_t max_short, pad_;
 } k2q_matrices;
 

@@ -40,10 +40,10 @@ struct Mat {            // one entry of the device table
   int32_t tile0, tiles;
 };
 static_assert(sizeof(Mat) == 48, "table layout");
-struct Tile { int32_t mat; int32_t pad; int64_t first; };   // columns [first, first + piece)
+struct Tile { int32_t mat; int32_t pad; int64_t first; };   // positions of the long side from `first` on
 
 struct StepParams {
-  const Mat* mats; const Tile* tiles; int64_t piece;
+  const Mat* mats; const Tile* tiles; int64_t piece;   // sub-blocks per piece
   float* p; float* g; float* m; float* out;
   float* ws;
   float lr, beta, wd, eps, max_norm;
@@ -185,7 +185,7 @@ __device__ __forceinline__ void gram_body(const StepParams& a, const Tile& tile,
   const Place pl(t, a.aligned, TALL, BLOCK);
   const Share sh(pl);
   const float clip = clip_factor(a);
-  const int64_t last = min(t.l, tile.first + a.piece);
+  const int64_t last = min(t.l, tile.first + a.piece * BLOCK);
   const int nt = pl.s4 >> 2, pairs = pairs_of(t.s), kgroups = kThreads / pairs;
   // this thread's tile (ti <= tj) and share of the positions
   const int kg = threadIdx.x / pairs, mine = threadIdx.x - kg * pairs;
@@ -465,7 +465,7 @@ __device__ __forceinline__ void apply_body(const StepParams& a, const Tile& tile
   const Place pl(t, a.aligned, TALL, BLOCK);
   const Share sh(pl);
   const float clip = clip_factor(a);
-  const int64_t last = min(t.l, tile.first + a.piece);
+  const int64_t last = min(t.l, tile.first + a.piece * BLOCK);
   const float rows = t.tall ? t.l : t.s, cols = t.tall ? t.s : t.l;
   const float step = a.lr * (a.scale_mode == 0 ? 0.2f * sqrtf(fmaxf(rows, cols)) : sqrtf(fmaxf(1.0f, rows / cols)));
   const float keep = 1.0f - a.lr * a.wd;
@@ -481,8 +481,11 @@ __device__ __forceinline__ void apply_body(const StepParams& a, const Tile& tile
   const float *am = pl.tall ? u : pm, *bm = pl.tall ? pm : u;
   const int ap = pl.tall ? pl.pitch : pp, bw = pl.tall ? pl.s4 : pl.width;
   const int rt = pl.rows >> 2, ct = pl.width >> 2;             // up to 256 tiles of 4 x 4
-  const int ri = threadIdx.x / ct, ci = (threadIdx.x - ri * ct) * 4;
-  const bool works = ri < rt;
+  // wide: eight threads side by side on a row, so that a warp's reads of B are four times one 128-byte line and not
+  // four whole rows of it (tall: B is P, with at most 16 tiles to a row)
+  const int strip = TALL ? ct : 8, in_strip = threadIdx.x % (rt * strip);
+  const int ri = in_strip / strip, ci = (threadIdx.x / (rt * strip) * strip + in_strip % strip) * 4;
+  const bool works = ci < pl.width;
 
   // raw pieces of this thread: g, m as the shares say, p where its results go
   float* raw = pm + up4(kMaxShort) * odd_pitch(up4(kMaxShort)) + threadIdx.x * 4;
@@ -626,17 +629,32 @@ int make_plan(const char* name, const int64_t* rows, const int64_t* cols, int64_
     pl.total += s * l;
     if (s > pl.max_short) pl.max_short = static_cast<int32_t>(s);
   }
-  // pieces of the long side: as long as they may be while the largest GPUs' SMs still get four of them each
-  const int64_t wanted = 4 * 148;
-  for (pl.piece = 2048; pl.piece > 128; pl.piece /= 2) {
+  // Sub-blocks per CTA: what fills whole waves best, two CTAs per SM in apply and three in gram, each with about 0.7
+  // sub-blocks' worth of start.  Measured on 58.7 M elements at rank 32: 16 per CTA (3.03 and 2.02 waves) 368 us, 8 (6.05
+  // and 4.04) 357, 10 (4.92 and 3.28, what this picks) 353.  The plan depends on the shapes alone, so the SM count is
+  // the B200's.
+  auto tiles_with = [&](int64_t per) {
     int64_t n = 0;
-    for (int64_t i = 0; i < count; ++i) n += ((rows[i] < cols[i] ? cols[i] : rows[i]) + pl.piece - 1) / pl.piece;
-    if (n >= wanted) break;
+    for (int64_t i = 0; i < count; ++i) {
+      const int64_t s = rows[i] < cols[i] ? rows[i] : cols[i], l = rows[i] < cols[i] ? cols[i] : rows[i];
+      const int64_t len = per * block_of(static_cast<int>(s));
+      n += (l + len - 1) / len;
+    }
+    return n;
+  };
+  double best = 0.0;
+  for (int64_t per = 1; per <= 32; ++per) {
+    const int64_t n = tiles_with(per);
+    const double waves = static_cast<double>((n + 2 * 148 - 1) / (2 * 148) + (n + 3 * 148 - 1) / (3 * 148)), cost = waves * (per + 0.7);
+    if (per == 1 || cost < best) {
+      best = cost;
+      pl.piece = per;
+    }
   }
   int64_t floats = 0;
   for (int64_t i = 0; i < count; ++i) {
     const int64_t s = rows[i] < cols[i] ? rows[i] : cols[i], l = rows[i] < cols[i] ? cols[i] : rows[i];
-    const int64_t n = (l + pl.piece - 1) / pl.piece;
+    const int64_t len = pl.piece * block_of(static_cast<int>(s)), n = (l + len - 1) / len;
     pl.tiles += n;
     const int32_t s32 = static_cast<int32_t>(s);
     floats += n * pairs_of(s32) * 16 + up4(s32) * up4(s32);
@@ -704,14 +722,15 @@ int k2q_matrices_table(const int64_t* rows, const int64_t* cols, int64_t count, 
     m.l = m.tall ? rows[i] : cols[i];
     m.off = off;
     m.tile0 = static_cast<int32_t>(nt);
-    m.tiles = static_cast<int32_t>((m.l + pl.piece - 1) / pl.piece);
+    const int64_t len = pl.piece * block_of(m.s);
+    m.tiles = static_cast<int32_t>((m.l + len - 1) / len);
     m.gram = floats;
     floats += static_cast<int64_t>(m.tiles) * pairs_of(m.s) * 16;
     m.poly = floats;
     floats += up4(m.s) * up4(m.s);
     off += m.s * m.l;
     mats[i] = m;
-    for (int k = 0; k < m.tiles; ++k) tiles[nt++] = Tile{static_cast<int32_t>(i), 0, k * pl.piece};
+    for (int k = 0; k < m.tiles; ++k) tiles[nt++] = Tile{static_cast<int32_t>(i), 0, k * len};
   }
   return K2Q_OK;
 }
