@@ -7,9 +7,9 @@
 // multiply-add each: the operations of the large W4A8 product on every element, so both give the same bits.
 // Bound by reading the codes once: N*K/2 bytes.
 //
-// A warp owns 8 or 16 channels over the whole contraction and folds every group in registers; nothing is
-// exchanged between warps.  A group of eight channels is four m16n8k32 int8 MMAs per 16 tokens, the tokens as
-// rows.  The order of k inside a group is free as long as both operands agree, so a lane simply takes 16
+// A warp owns 8 or 16 channels and folds its groups in registers.  A group of eight channels is four m16n8k32 int8 MMAs
+// per 16 tokens, the tokens as rows (dp4a reaches a quarter of their rate, and needs the codes as bytes as well).  The
+// order of k inside a group is free as long as both operands agree, so a lane simply takes 16
 // consecutive bytes of a channel (32 codes): the low nibbles of a word, shifted up, and its high nibbles are two
 // operand registers holding 16 times the codes, and the tokens' bytes are dealt out to match (even and odd
 // bytes of eight).
@@ -17,7 +17,15 @@
 //     only what it copied itself, so the ring needs no barrier and stays full whatever the arithmetic does.
 //   - The tokens and the scales are staged in shared memory beforehand.  Plain loads of them inside the loop return
 //     in order behind the codes' misses in the L1 pipe and cost each group a trip to DRAM (measured: 520 ns a
-//     group); copies of them in the ring, several lanes from one address, were slower still.
+//     group); copies of them in the ring, several lanes from one address, were slower still (53 us against 24 to 31 at 16
+//     rows, 6144 channels, K = 16384).  Two warps set aside to bring the tokens chunk by chunk took 46 us there, 29 without
+//     them (the MMA order changed between the two as well).
+// One CTA per SM, so that the tokens are staged once per SM.  With few channels per SM, several warps share eight
+// channels and pass the running values on in block order (ring kernel below).
+// Measured on a B200 (codes from DRAM): 36864 x 6144 23.0 / 25.2 / 27.0 us at 1 / 8 / 16 rows (reading the codes and scales
+// at the copy bandwidth: 17.8), 6144 x 6144 7.9 / 9.2 / 11.8 (3.0), 6144 x 16384 14.8 / 19.2 / 27.3 (7.9), 6144 x 256
+// 3.0 / 3.4 / 3.8 (0.1).  With 13 rows of K = 16384 the ring kernel runs 12 warps per SM, issues in 46 % of the cycles
+// and reads DRAM at 23 % of its peak: instruction latency and shared memory, not the codes.
 #include "k2q_common.cuh"
 
 namespace k2q {

@@ -12,7 +12,7 @@
 //   gram    m' and the partial Gram matrices of pieces of the long side       12 B and S/2 FMA per element
 //   poly    partials added, normalised, iterated; leaves P = (Q ... Q_0) / (||u||_F + eps)
 //   apply   P u and the parameter step                                        16 B and S FMA per element
-// gram and apply are bound by HBM up to S = 32 and by the fp32 pipe beyond.  Both work on sub-blocks of 4096 elements in
+// Up to S = 32 gram and apply are nearest to HBM, beyond to shared memory.  Both work on sub-blocks of 4096 elements in
 // shared memory with 4 x 4 register tiles and packed fp32 pairs: a pair holds two neighbouring positions of the
 // CONTRACTED index, so no operand has to be broadcast and one instruction does two multiply-adds.  Where that index
 // is the contiguous one in memory (gram of a wide matrix, apply of a tall one) the sub-block stays as it is
@@ -21,6 +21,12 @@
 // The S x S iteration is in 64 bits, on the fp64 tensor instructions (8 x 8 tiles of the upper triangle): P's entries reach a^steps, so what G_0 loses to rounding comes back up to
 // that much larger in the weak directions.  G_0's products are summed in fp32 by each thread over its share of a piece
 // (a few hundred terms), over threads in fp32, over pieces in 64 bits.  All sums run in a fixed order.
+// Measured on a B200 (copy bandwidth 6.55 TB/s), 224 adapter matrices, 58.7 M elements:
+//   rank 32   353 us in all (launched one by one: gram 139, poly 25, apply 200).  20 B per element, which a single pass
+//             could not do without, would take 179 us, the 28 B of two passes 251
+//   rank 16   144 us for 22 M elements (67 at 20 B each)      rank 64, half the matrices, 58.7 M elements   568 us
+// At rank 64 shared memory is busiest: 63 % of its rate in gram and apply, with DRAM near 30 and the fp32 pipe at 28 %; gram
+// waits most at its barriers.  The iteration takes 52 us there, on one SM per matrix.
 #include "k2q_common.cuh"
 
 namespace k2q {

@@ -555,8 +555,8 @@ def gemm_w4a8(xq, sx, wq4, sw4, bias=None, u=None, bm=None, lora_scale: float = 
 GEMV_ROWS = 32        # token rows that gemv_w4a8 takes
 GEMV_MAX_K = 131072
 # Rows that gemm_w4a8 hands to it.  Measured on a B200 with weights from DRAM, few-row kernel against the large
-# product's: 16 rows 27.0 / 68.8 us at 36864 x 6144, 12.6 / 27.6 at 6144 x 6144, 18.4 / 37.0 at 16384 x 6144, 3.8 / 5.8
-# at 6144 x 256; 32 rows 42.6 / 52.5, 20.2 / 27.3, 29.4 / 28.0, 5.3 / 5.8 -- between the two the large product's tiles
+# product's: 16 rows 27.0 / 68.8 us at 36864 x 6144, 11.8 / 27.6 at 6144 x 6144, 18.4 / 37.0 at 16384 x 6144, 3.8 / 5.8
+# at 6144 x 256; 32 rows 43.3 / 52.3, 20.7 / 27.2, 29.7 / 28.0, 5.3 / 5.8 -- between the two the large product's tiles
 # start to fill the SMs, and the few-row kernel's token reads to cost as much as the codes.
 GEMV_BEST_ROWS = 16
 
