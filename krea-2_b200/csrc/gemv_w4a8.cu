@@ -88,7 +88,7 @@ constexpr int kMaxWarps = 16;
 // named barriers (0 is __syncthreads)
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-constexpr int kSmemMax = 232448;
+constexpr int kSmemMax = 232448;      // also every kernel's limit, whatever the launch needs: launches of other threads share it
 
 // Groups [g0, g0 + chunk) of every token into shared memory, the even and the odd bytes of every eight apart.  A
 // token's row there is chunk * 128 + 16 bytes long: the eight lanes of a 16-byte read phase (two tokens, four
@@ -408,7 +408,7 @@ int launch_ring(GemvParams p, int teams, int ks, cudaStream_t stream) {
   p.ks = ks;
   const int smem = fixed + p.M * (p.chunk * 128 + 16);
   auto kern = gemv_ring_kernel<MH, RING>;
-  if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+  if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax),
                           "cudaFuncSetAttribute(gemv_w4a8)"))
     return rc;
   const int tiles = p.N / 8, all = warps > 8 ? warps : 8;      // eight warps at least stage the tokens
@@ -425,7 +425,7 @@ int launch_one(GemvParams p, int warps, cudaStream_t stream) {
   p.chunk = chunk < groups ? chunk : (groups + GP - 1) / GP * GP;
   const int smem = fixed + p.M * (p.chunk * 128 + 16);
   auto kern = gemv_kernel<MH, CT, GP, RING>;
-  if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+  if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax),
                           "cudaFuncSetAttribute(gemv_w4a8)"))
     return rc;
   p.warps = warps;

@@ -686,12 +686,14 @@ int run_steps(const char* name, const k2q_matrices* pl, const void* table, StepP
   a.aligned = !off16(a.p) && !off16(a.g) && !off16(a.m) && !off16(a.out);
   const int s4 = up4(pl->max_short);
   const int poly_smem = 4 * up8(pl->max_short) * pitch64(pl->max_short) * 8;
+  const int poly_widest = pl->max_short <= 32 ? 32 : kMaxShort;      // the limit is the kernel's: launches of other threads share it
+  const int poly_limit = 4 * up8(poly_widest) * pitch64(poly_widest) * 8;
   const int apply_smem = (kMaxSub + up4(kMaxShort) * odd_pitch(up4(kMaxShort))) * 4 + 3 * kRaw;
   if (int rc = check_cuda(cudaFuncSetAttribute(gram_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGramSmem),
                           "cudaFuncSetAttribute(gram)"))
     return rc;
   auto poly = pl->max_short <= 32 ? poly_kernel<8, 2> : poly_kernel<16, 3>;
-  if (int rc = check_cuda(cudaFuncSetAttribute(poly, cudaFuncAttributeMaxDynamicSharedMemorySize, poly_smem),
+  if (int rc = check_cuda(cudaFuncSetAttribute(poly, cudaFuncAttributeMaxDynamicSharedMemorySize, poly_limit),
                           "cudaFuncSetAttribute(poly)"))
     return rc;
   if (int rc = check_cuda(cudaFuncSetAttribute(apply_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, apply_smem),

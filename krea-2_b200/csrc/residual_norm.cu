@@ -654,13 +654,17 @@ int chunks_for(int64_t B, int64_t rows_per_batch, int ctas_per_sm) {
   return static_cast<int>(c < 1 ? 1 : c);
 }
 using Kernel = void (*)(ResParams);
-// CTAs of a kernel that share an SM, asked of the runtime once per kernel (`slot`) and number of warps
-int ctas_per_sm(Kernel kern, int slot, int threads, int smem) {
+// Shared memory limits are a kernel's, not a launch's: always the largest that it can need, so that a host thread never
+// lowers the limit between another one's setting it and launching.
+constexpr int kQuantSmem = 16384 * 8, kBwdSmem = 16384 * 12;
+// CTAs of a kernel that share an SM, asked of the runtime once per kernel (`slot`) and number of warps; `smem` belongs to
+// the widest row of that number of warps, so that the grid does not depend on which row came first
+int ctas_per_sm(Kernel kern, int slot, int threads, int smem, int limit) {
   static std::atomic<int> known[16][17];
   std::atomic<int>& k = known[slot][threads / 32];
   int n = k.load(std::memory_order_relaxed);
   if (n == 0) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, limit) != cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, static_cast<size_t>(smem)) != cudaSuccess || n < 1) {
       cudaGetLastError();
       return 1;
@@ -691,7 +695,8 @@ BwdShape bwd_shape(int64_t B, int64_t rows_per_batch, int64_t K, bool sums) {
   dense_shape(K, &s.threads, &vpt);
   s.slot = (vpt - 1) * 2 + (sums ? 1 : 0);
   s.smem = sums && vpt > 1 ? static_cast<int>(K) * 12 : 0;
-  s.chunks = chunks_for(B, rows_per_batch, ctas_per_sm(kBwd[s.slot], s.slot, s.threads, s.smem));
+  const int widest = s.smem > 0 ? s.threads * vpt * 8 * 12 : 0;
+  s.chunks = chunks_for(B, rows_per_batch, ctas_per_sm(kBwd[s.slot], s.slot, s.threads, widest, s.smem > 0 ? kBwdSmem : 0));
   return s;
 }
 
@@ -723,11 +728,11 @@ int k2q_residual_norm_quant(const void* x_bf16, int64_t ldx, const void* y_bf16,
     return fail(K2Q_EINVAL, "%s: rows must be 16-byte aligned with a leading dimension >= K", name);
   const int threads = (static_cast<int>(K / 32) + 31) / 32 * 32;
   const int64_t B = M / rows_per_batch;
-  const int vec_bytes = static_cast<int>(K) * (4 + (p.mshift ? 2 : 0) + (p.gate ? 2 : 0));
+  const int per_k = 4 + (p.mshift ? 2 : 0) + (p.gate ? 2 : 0), vec_bytes = static_cast<int>(K) * per_k;
   const int slot = (p.gate ? 2 : 0) + (p.mshift ? 1 : 0);
-  p.chunks = chunks_for(B, rows_per_batch, ctas_per_sm(kQuant[slot], 12 + slot, threads, vec_bytes));
+  p.chunks = chunks_for(B, rows_per_batch, ctas_per_sm(kQuant[slot], 12 + slot, threads, threads * 32 * per_k, kQuantSmem));
   if (B * p.chunks > 0x7fffffffLL) return fail(K2Q_EINVAL, "%s: too many samples (%lld)", name, (long long)B);
-  if (int rc = check_cuda(cudaFuncSetAttribute(kQuant[slot], cudaFuncAttributeMaxDynamicSharedMemorySize, vec_bytes),
+  if (int rc = check_cuda(cudaFuncSetAttribute(kQuant[slot], cudaFuncAttributeMaxDynamicSharedMemorySize, kQuantSmem),
                           "cudaFuncSetAttribute(residual_quant)"))
     return rc;
   return launch_overlapped(kQuant[slot], static_cast<unsigned>(B * p.chunks), static_cast<unsigned>(threads), static_cast<size_t>(vec_bytes),
@@ -757,7 +762,7 @@ int k2q_residual_norm_fwd(const void* x_bf16, int64_t ldx, const void* y_bf16, i
   int threads, vpt;
   dense_shape(K, &threads, &vpt);
   const int64_t B = M / rows_per_batch;
-  p.chunks = chunks_for(B, rows_per_batch, ctas_per_sm(kFwd[vpt - 1], 8 + vpt - 1, threads, 0));
+  p.chunks = chunks_for(B, rows_per_batch, ctas_per_sm(kFwd[vpt - 1], 8 + vpt - 1, threads, 0, 0));
   if (B * p.chunks > 0x7fffffffLL) return fail(K2Q_EINVAL, "%s: too many samples (%lld)", name, (long long)B);
   return launch_overlapped(kFwd[vpt - 1], static_cast<unsigned>(B * p.chunks), static_cast<unsigned>(threads), 0,
                            static_cast<cudaStream_t>(stream), 1, "residual_fwd launch", p);
@@ -809,7 +814,7 @@ int k2q_residual_norm_bwd(const void* dstream_bf16, int64_t ldds, const void* dh
   if (B * p.chunks > 0x7fffffffLL) return fail(K2Q_EINVAL, "%s: too many samples (%lld)", name, (long long)B);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (shape.smem > 0) {
-    if (int rc = check_cuda(cudaFuncSetAttribute(kBwd[shape.slot], cudaFuncAttributeMaxDynamicSharedMemorySize, shape.smem),
+    if (int rc = check_cuda(cudaFuncSetAttribute(kBwd[shape.slot], cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdSmem),
                             "cudaFuncSetAttribute(residual_bwd)"))
       return rc;
   }

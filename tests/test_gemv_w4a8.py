@@ -133,3 +133,31 @@ def test_refusals_on_gpu():
         ops.gemv_w4a8(xq[:2], sx[:2], wq[:24], sw[:24], None)                    # N not a multiple of 16
     with pytest.raises(ValueError):
         ops.gemv_w4a8(xq[:2], sx[:2], wq, sw, b, u=torch.zeros(2, 33, device="cuda"), bm=torch.zeros(32, 33, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_two_host_threads():
+    """Calls of very different shared memory needs from two threads at once: a kernel's limit serves both."""
+    import threading
+    small, large = make(1, 64, 2560, 1), make(8, 64, 16384, 2)            # one kernel, 20 and 200 KB
+    want = [ops.gemv_w4a8(*c) for c in (small, large)]
+    torch.cuda.synchronize()
+    errors, start = [], threading.Barrier(2)
+
+    def work(c, w):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait(timeout=30)
+                for _ in range(4000):
+                    y = ops.gemv_w4a8(*c)
+                torch.cuda.current_stream().synchronize()
+                assert same_bits(y, w)
+        except Exception as e:      # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=cw) for cw in zip((small, large), want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
