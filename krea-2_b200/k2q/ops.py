@@ -776,6 +776,8 @@ def orthogonal_step_(param: torch.Tensor, grad: torch.Tensor, moment: torch.Tens
         raise ValueError(f"{name}: scale must be one of {sorted(_STEP_SCALES)}, got {scale!r}")
     if normsq is not None and (normsq.dtype != torch.float32 or normsq.numel() != 1 or normsq.device != dev):
         raise ValueError(f"{name}: normsq must be one fp32 value on the buffers' device")
+    if normsq is None and max_norm > 0:
+        raise ValueError(f"{name}: clipping to max_norm needs normsq")
     pl = layout.plan
     ws = torch.empty(pl.workspace_bytes // 4, dtype=torch.float32, device=dev)
     _launch(dev, _lib.load().k2q_orthogonal_step, "k2q_orthogonal_step", param.data_ptr(), grad.data_ptr(), moment.data_ptr(),

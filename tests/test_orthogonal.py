@@ -213,3 +213,12 @@ def test_refusals_on_gpu():
             ops.orthogonal_step_(p, g, m, layout, lr=0.1, **kw)
     with pytest.raises(ValueError):
         ops.orthogonalize(big[:550], layout, out=big[100:650])
+
+
+@pytest.mark.gpu
+def test_clipping_needs_the_norm():
+    layout = ops.MatrixLayout([(4, 100)], "cuda")
+    p, g, m = (torch.ones(400, device="cuda") for _ in range(3))
+    with pytest.raises(ValueError, match="normsq"):
+        ops.orthogonal_step_(p, g, m, layout, lr=0.1, max_norm=1.0)
+    assert all(torch.equal(t, torch.ones_like(t)) for t in (p, g, m))
