@@ -140,3 +140,23 @@ def test_orthogonal_step_refuses_vectors_and_large_ranks():
         p = torch.nn.Parameter(torch.zeros(shape, device="cuda"))
         with pytest.raises(ValueError):
             trainer.FusedOrthogonalStep(parallel.AdapterGradBuckets([[p]]))
+
+
+def test_time_path_is_saved_and_loaded_with_the_base(tmp_path):
+    from k2q import dit, modules, serialize
+    make = lambda: dit.SingleStreamDiT(dit.DiTConfig(**CFG)).to(torch.bfloat16).cuda()      # noqa: E731
+    m = make()
+    n = modules.quantize_dit_convrot(m, bits=4, backward_copy=False) + modules.quantize_time_path(m)
+    assert modules.quantize_time_path(m) == 0                    # nothing is quantised twice
+    path = str(tmp_path / "base.safetensors")
+    assert serialize.save_quantized_base(m, path) == n
+    fresh = make()
+    assert serialize.load_quantized_base(fresh, path, device="cuda") == n
+    for name, want in serialize.convrot_modules(m).items():
+        got = fresh.get_submodule(name)
+        assert torch.equal(got.weight_q, want.weight_q) and torch.equal(got.scale, want.scale)
+    mixed = make()
+    modules.quantize_dit_convrot(mixed, bits=8)
+    modules.quantize_time_path(mixed, bits=4)
+    with pytest.raises(ValueError, match="mixed bit widths"):
+        serialize.save_quantized_base(mixed, path)

@@ -222,3 +222,19 @@ def test_clipping_needs_the_norm():
     with pytest.raises(ValueError, match="normsq"):
         ops.orthogonal_step_(p, g, m, layout, lr=0.1, max_norm=1.0)
     assert all(torch.equal(t, torch.ones_like(t)) for t in (p, g, m))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [1, 19, 75])
+def test_few_and_many_matrices_of_large_rank(count):
+    """A matrix's result does not depend on how many stand beside it (one piece per matrix, so that its Gram sums
+    are formed in one order)."""
+    kinds = [(33, 50), (64, 64), (61, 57), (40, 41), (5, 64)]
+    shapes = [kinds[i % 5] for i in range(count)]
+    mats = [matrix(r, c, i) for i, (r, c) in enumerate(kinds)]
+    flat = torch.cat([mats[i % 5].reshape(-1) for i in range(count)])
+    got = ops.orthogonalize(flat, ops.MatrixLayout(shapes, "cuda")).split([r * c for r, c in shapes])
+    many = torch.cat([m.reshape(-1) for m in mats]).repeat(32)                   # 160 matrices
+    want = ops.orthogonalize(many, ops.MatrixLayout(kinds * 32, "cuda")).split([r * c for r, c in kinds * 32])
+    for i in range(count):
+        assert torch.equal(got[i], want[i % 5]), shapes[i]
