@@ -12,7 +12,7 @@
 //   gram    m' and the partial Gram matrices of pieces of the long side       12 B and S/2 FMA per element
 //   poly    partials added, normalised, iterated; leaves P = (Q ... Q_0) / (||u||_F + eps)
 //   apply   P u and the parameter step                                        16 B and S FMA per element
-// Up to S = 32 gram and apply are nearest to HBM, beyond to shared memory.  Both work on sub-blocks of 4096 elements in
+// Neither saturates one unit (figures below): shared memory is the busiest.  Both work on sub-blocks of 4096 elements in
 // shared memory with 4 x 4 register tiles and packed fp32 pairs: a pair holds two neighbouring positions of the
 // CONTRACTED index, so no operand has to be broadcast and one instruction does two multiply-adds.  Where that index
 // is the contiguous one in memory (gram of a wide matrix, apply of a tall one) the sub-block stays as it is
@@ -25,8 +25,10 @@
 //   rank 32   353 us in all (launched one by one: gram 139, poly 25, apply 200).  20 B per element, which a single pass
 //             could not do without, would take 179 us, the 28 B of two passes 251
 //   rank 16   144 us for 22 M elements (67 at 20 B each)      rank 64, half the matrices, 58.7 M elements   568 us
-// At rank 64 shared memory is busiest: 63 % of its rate in gram and apply, with DRAM near 30 and the fp32 pipe at 28 %; gram
-// waits most at its barriers.  The iteration takes 52 us there, on one SM per matrix.
+// Counters of gram / apply at rank 32: shared memory 61 / 55 % of its rate, issue 57 / 52 %, DRAM 54 / 49 %, fp32 pipe 27 / 24 %,
+// at 21 / 15 warps per SM: latency between units that are each half busy.  Taking apply's pieces backwards, to find the
+// last of gram's in L2, saved 5 % of its reads and 0.4 % of the time, and is not done.  At rank 64: shared memory 63 / 63 %,
+// DRAM 29 / 32 %, fp32 pipe 28 / 28 %; gram waits most at its barriers.  The iteration takes 52 us there, on one SM per matrix.
 #include "k2q_common.cuh"
 
 namespace k2q {
