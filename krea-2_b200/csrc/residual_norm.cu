@@ -13,7 +13,7 @@
 //
 // Everything between the loads and the stores is fp32; the stream is rounded to bf16 once, where it is
 // kept, and the norm reads the rounded values, so that the backward sees the same numbers.  b = row /
-// rows_per_batch.  All three are bound by HBM: 7, 8 and 10 (12 with the sums) bytes per element.  A row is worked on by
+// rows_per_batch.  They move 7, 8 and 10 (12 with the sums) bytes per element; the forward and the backward without sums are held by HBM, the others by what follows.  A row is worked on by
 // one CTA (its two reductions are CTA-wide); a CTA takes consecutive rows of one sample, so that the sample's vectors are
 // read from L2 once per CTA and not once per row, and there are exactly as many CTAs as the SMs hold at once.  The
 // quantising kernel is held to 96 registers, so that three CTAs of 192 threads fit (at 124, two did, in 1.5 waves): that,
