@@ -116,16 +116,6 @@ struct Smem4 {
   static constexpr uint32_t kBytes = kBarOff + kNumBars * 8 + 16;
 };
 
-__device__ __forceinline__ float gelu_tanh4(float v) {
-  // 0.5 v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) with the hardware tanh (|error| < 6e-4, far below
-  // the bf16 resolution of the output)
-  const float z = v * fmaf(0.0356774081f, v * v, 0.7978845608f);
-  float th;
-  asm("tanh.approx.f32 %0, %1;" : "=f"(th) : "f"(z));
-  const float hv = 0.5f * v;
-  return fmaf(hv, th, hv);
-}
-
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   uint32_t r;
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
@@ -155,11 +145,14 @@ __device__ __forceinline__ void finish_tile(const uint64_t* run2, const float* s
     float rv[2];
     unpack_f32x2(run2[j2], rv[0], rv[1]);
 #pragma unroll
+    for (int e = 0; e < 2; ++e) rv[e] = __fadd_rn(__fmul_rn(rv[e], sxp[2 * j2 + e]), bias_n);
+    if (GELU) {
+      const uint64_t a2 = gelu_tanh2(pack_f32x2(rv[0], rv[1]));
+      unpack_f32x2(a2, rv[0], rv[1]);
+    }
+#pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int jl = 2 * j2 + e;
-      float tv = __fadd_rn(__fmul_rn(rv[e], sxp[jl]), bias_n);
-      if (GELU) tv = gelu_tanh4(tv);
-      if (jl < valid) *yp = __float2bfloat16_rn(tv);
+      if (2 * j2 + e < valid) *yp = __float2bfloat16_rn(rv[e]);
       yp += ldy;
     }
   }
@@ -490,7 +483,7 @@ gemm_w4a8_kernel(const __grid_constant__ CUtensorMap tmap_w4, const __grid_const
             const int j = ch * CW + 2 * j2 + e;
             float tv = __fmul_rn(rv[e], sx_s[j]);
             tv = __fadd_rn(tv, bias_n);
-            if (p.act == K2Q_ACT_GELU_TANH) tv = gelu_tanh4(tv);
+            if (p.act == K2Q_ACT_GELU_TANH) tv = gelu_tanh(tv);
             const float4* u4 = reinterpret_cast<const float4*>(u_s + j * RD);
             float d = 0.f;
 #pragma unroll

@@ -82,16 +82,6 @@ struct Smem {
   static constexpr uint32_t kBytes = kBarOff + (2 * STAGES + 4) * 8 + 16;
 };
 
-__device__ __forceinline__ float gelu_tanh_f(float v) {
-  // 0.5 v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) with the hardware tanh (|error| < 6e-4, far below
-  // the bf16 resolution of the output)
-  const float z = v * fmaf(0.0356774081f, v * v, 0.7978845608f);
-  float th;
-  asm("tanh.approx.f32 %0, %1;" : "=f"(th) : "f"(z));
-  const float hv = 0.5f * v;
-  return fmaf(hv, th, hv);
-}
-
 template <int STAGES, int RMAX, bool PAIR, bool BMN, bool FMA>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_w8a8_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
@@ -406,8 +396,14 @@ gemm_w8a8_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
             float t = __fmul_rn(static_cast<float>(static_cast<int32_t>(acc[j])), sxr);
             t = __fmul_rn(t, sw_s[cj]);
             t = __fadd_rn(t, bias_s[cj]);
-            if (p.act == K2Q_ACT_GELU_TANH) t = gelu_tanh_f(t);
             v[j] = t;
+          }
+          if (p.act == K2Q_ACT_GELU_TANH) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const uint64_t a2 = gelu_tanh2(pack_f32x2(v[j], v[j + 1]));
+              unpack_f32x2(a2, v[j], v[j + 1]);
+            }
           }
           if (row_ok) {
 #pragma unroll
@@ -469,10 +465,10 @@ gemm_w8a8_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
               float t = __fmul_rn(static_cast<float>(static_cast<int32_t>(acc[2 * j + h])), sxr);
               t = __fmul_rn(t, sw_s[cj]);
               t = __fadd_rn(t, bias_s[cj]);
-              if (p.act == K2Q_ACT_GELU_TANH) t = gelu_tanh_f(t);
               tv[h] = t;
             }
             t2[j] = pack_f32x2(tv[0], tv[1]);
+            if (p.act == K2Q_ACT_GELU_TANH) t2[j] = gelu_tanh2(t2[j]);
           }
 #pragma unroll
           for (int j = 0; j < RD; ++j) {
@@ -611,8 +607,8 @@ gemm_w8a8_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
                 t0 = __fadd_rn(__fmul_rn(t0, sw2.x), bi2.x);
                 t1 = __fadd_rn(__fmul_rn(t1, sw2.y), bi2.y);
                 if (p.act == K2Q_ACT_GELU_TANH) {
-                  t0 = gelu_tanh_f(t0);
-                  t1 = gelu_tanh_f(t1);
+                  const uint64_t a2 = gelu_tanh2(pack_f32x2(t0, t1));
+                  unpack_f32x2(a2, t0, t1);
                 }
                 pk[h] = pack_bf16x2(t0 + cf[mt][nt][2 * h], t1 + cf[mt][nt][2 * h + 1]);
               }

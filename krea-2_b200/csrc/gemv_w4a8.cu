@@ -45,18 +45,9 @@ struct GemvParams {
   int chunk;                          // groups of the tokens staged at a time
 };
 
-// the activation of the large product: hardware tanh, |error| < 6e-4, below the bf16 step of the output
-__device__ __forceinline__ float gelu_tanh_hw(float v) {
-  const float z = v * fmaf(0.0356774081f, v * v, 0.7978845608f);
-  float th;
-  asm("tanh.approx.f32 %0, %1;" : "=f"(th) : "f"(z));
-  const float hv = 0.5f * v;
-  return fmaf(hv, th, hv);
-}
-
 __device__ __forceinline__ void finish(const GemvParams& p, int m, int n, float run) {
   float v = __fadd_rn(__fmul_rn(run, p.sx != nullptr ? __ldg(p.sx + m) : 1.0f), p.bias != nullptr ? __ldg(p.bias + n) : 0.0f);
-  if (p.act == K2Q_ACT_GELU_TANH) v = gelu_tanh_hw(v);
+  if (p.act == K2Q_ACT_GELU_TANH) v = gelu_tanh(v);
   if (p.rank > 0) {
     float d = 0.f;
     for (int j = 0; j < p.rank; ++j)
