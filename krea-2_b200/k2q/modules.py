@@ -479,7 +479,7 @@ def quantize_dit_convrot(dit, bits: int = 8, group: int = GROUP, had_block: int 
 def fuse_residual_norms(dit, fused: bool = True) -> int:
     """Makes the blocks of a :class:`~k2q.dit.SingleStreamDiT` (its text-fusion blocks too) run the stream's update
     behind the attention and the norm in front of the MLP as one step, in training and in sampling
-    (``fused.residual_norm``, ``ops.residual_norm_quant``).  That step is fp32 inside where the single kernels
+    (``fused.residual_norm``, ``ops.residual_norm_quant``), before or after the model is split over GPUs.  That step is fp32 inside where the single kernels
     round to bf16 after every operation as the reference's eager code does, so results differ in
     their last bits; ``fused=False`` goes back.  Returns the number of blocks switched."""
     n = 0

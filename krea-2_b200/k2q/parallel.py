@@ -345,10 +345,13 @@ class ColumnParallelBlock(nn.Module):
     """``SingleStreamBlock`` (mmdit.py:258-276) under the column split with local attention: the residual
     stream and both norms are replicated, every Linear is a column shard, and four all-gathers per block
     (gated attention output, ``wo`` output, SwiGLU product, ``down`` output) replace the eight of a
-    Linear-by-Linear split.  Bit-identical with the unsharded block."""
+    Linear-by-Linear split.  Bit-identical with the unsharded block, fused residual steps included."""
+
+    residual_fused = False                    # ``modules.fuse_residual_norms``, before or after the split
 
     def __init__(self, block: nn.Module, rank: int, world: int, group=None):
         super().__init__()
+        self.residual_fused = getattr(block, "residual_fused", False)
         self.mod, self.prenorm, self.postnorm = block.mod, block.prenorm, block.postnorm
         self.attn = ColumnLocalAttention(block.attn, rank, world, group)
         self.mlp = ColumnLocalSwiGLU(block.mlp, rank, world, group)
@@ -359,9 +362,17 @@ class ColumnParallelBlock(nn.Module):
         if fused_prologue_ok(x, a.wq, a.wk, a.wv, a.gate, m.gate, m.up):
             lead = x.shape[:2]
             xq, sx = ops.norm_mod_quant(x, self.prenorm.scale.float(), prescale, preshift, self.prenorm.eps)
+            if self.residual_fused:
+                x, xq, sx = ops.residual_norm_quant(x, a.forward_codes(xq, sx, lead, rope, mask), self.postnorm.scale.float(),
+                                                    pregate, postscale, postshift, self.postnorm.eps)
+                return gate_residual(x, postgate, m.forward_codes(xq, sx, lead))
             x = gate_residual(x, pregate, a.forward_codes(xq, sx, lead, rope, mask))
             xq, sx = ops.norm_mod_quant(x, self.postnorm.scale.float(), postscale, postshift, self.postnorm.eps)
             return gate_residual(x, postgate, m.forward_codes(xq, sx, lead))
+        if self.residual_fused:
+            x, h = fused.residual_norm(x, a(fused.norm_modulate(x, self.prenorm, prescale, preshift), rope, mask),
+                                       self.postnorm.scale.float(), pregate, postscale, postshift, self.postnorm.eps)
+            return gate_residual(x, postgate, m(h))
         x = gate_residual(x, pregate, a(fused.norm_modulate(x, self.prenorm, prescale, preshift), rope, mask))
         return gate_residual(x, postgate, m(fused.norm_modulate(x, self.postnorm, postscale, postshift)))
 
@@ -640,8 +651,11 @@ class SequenceParallelBlock(nn.Module):
     a token-sharded residual stream.  The first block of the stack takes the full sequence and keeps its
     slice, the last one gathers the slices again; in between only slices are passed on."""
 
+    residual_fused = False                    # ``modules.fuse_residual_norms``, before or after the split
+
     def __init__(self, block: nn.Module, rank: int, world: int, group=None, first=False, last=False):
         super().__init__()
+        self.residual_fused = getattr(block, "residual_fused", False)
         self.rank, self.world, self.group, self.first, self.last = rank, world, group, first, last
         self.mod, self.prenorm, self.postnorm = block.mod, block.prenorm, block.postnorm
         self.attn = HeadParallelAttention(block.attn, rank, world, group)
@@ -684,17 +698,27 @@ class SequenceParallelBlock(nn.Module):
             tl = t // self.world
             x = x[:, self.rank * tl:(self.rank + 1) * tl]
         prescale, preshift, pregate, postscale, postshift, postgate = self.mod(vec)
-        fused = not torch.is_grad_enabled() and x.is_cuda and x.dtype == torch.bfloat16
+        kernels = not torch.is_grad_enabled() and x.is_cuda and x.dtype == torch.bfloat16
 
         def codes_of(x_, norm, scale, shift):
             x_ = x_.contiguous()
             return lambda: (*ops.norm_mod_quant(x_, norm.scale.float(), scale, shift, norm.eps), tuple(x_.shape))
 
-        n = codes_of(x, self.prenorm, prescale, preshift) if (fused and self.codes_attn) else \
+        n = codes_of(x, self.prenorm, prescale, preshift) if (kernels and self.codes_attn) else \
             (1 + prescale) * self.prenorm(x) + preshift
-        x = gate_residual(x.contiguous(), pregate, self._my_tokens(self.attn(self._all_tokens(n, self.codes_attn), rope, mask)))
-        n = codes_of(x, self.postnorm, postscale, postshift) if (fused and self.codes_mlp) else \
-            (1 + postscale) * self.postnorm(x) + postshift
+        x = x.contiguous()
+        y = self._my_tokens(self.attn(self._all_tokens(n, self.codes_attn), rope, mask))
+        if self.residual_fused:
+            step = (x, y, self.postnorm.scale.float(), pregate, postscale, postshift, self.postnorm.eps)
+            if kernels and self.codes_mlp:
+                x, xq, sx = ops.residual_norm_quant(*step)
+                n = lambda: (xq, sx, tuple(x.shape))                                   # noqa: E731
+            else:
+                x, n = fused.residual_norm(*step)
+        else:
+            x = gate_residual(x, pregate, y)
+            n = codes_of(x, self.postnorm, postscale, postshift) if (kernels and self.codes_mlp) else \
+                (1 + postscale) * self.postnorm(x) + postshift
         x = gate_residual(x, postgate, self._my_tokens(self.mlp(self._all_tokens(n, self.codes_mlp))))
         if self.last:
             self.gathered_bytes += (self.world - 1) * x.numel() * x.element_size()
