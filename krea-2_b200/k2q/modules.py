@@ -490,12 +490,17 @@ def fuse_residual_norms(dit, fused: bool = True) -> int:
     return n
 
 
-def quantize_time_path(dit, bits: int = 4, group: int = GROUP, had_block: int = HAD_BLOCK) -> int:
+def quantize_time_path(dit, bits: int | None = None, group: int = GROUP, had_block: int = HAD_BLOCK) -> int:
     """Replaces the Linears of the timestep MLP and of the modulation projection (``tmlp``, ``tproj``, mmdit.py:360-375), which
     :func:`quantize_dit_convrot` leaves in bf16, with :class:`ConvRotLinear`; returns how many were replaced.  They
-    see one row per image: with ``bits=4`` such a product is one reading of the 4-bit codes (``ops.gemv_w4a8``),
-    a quarter of the bf16 weights' bytes in memory and per step.  The path is frozen (no backward copy); sampling and
-    adapter training both run through it."""
+    see one row per image: with 4 bits such a product is one reading of the codes (``ops.gemv_w4a8``), a quarter of the
+    bf16 weights' bytes in memory and per step.  The path is frozen (no backward copy); sampling and adapter training
+    both run through it.  Without ``bits`` it takes the width of the Linears quantised already (4 where there are none or
+    of several widths): ``serialize.save_quantized_base`` writes bases of one width only, so a model that is to be saved
+    keeps to that."""
+    if bits is None:
+        widths = {m.bits for m in dit.modules() if isinstance(m, ConvRotLinear)}
+        bits = widths.pop() if len(widths) == 1 else 4
     targets = [(seq, name, child) for seq in (dit.tmlp, dit.tproj) for name, child in seq.named_children()
                if isinstance(child, nn.Linear)]
     for _, name, child in targets:             # all or none
