@@ -32,6 +32,13 @@ def note_raw_write() -> None:
 def raw_write_epoch() -> int:
     return _raw_writes
 
+
+def _note_written(*tensors: torch.Tensor) -> None:
+    """:func:`note_raw_write` for tensors that a graph may have saved: it must not read the new values unnoticed."""
+    note_raw_write()
+    torch.autograd.graph.increment_version(tensors)        # (inference tensors have no version: left alone)
+
+
 _status_blocks: dict[int, torch.Tensor] = {}
 
 
@@ -359,9 +366,7 @@ def residual_norm_quant(x: torch.Tensor, y: torch.Tensor, norm_scale: torch.Tens
         for what, p, ld in (("x", xp, ldx), ("y", yp, ldy)):
             if op < p + ((m - 1) * ld + k) * 2 and p < op + ((m - 1) * ldo + k) * 2 and not (op == p and ldo == ld):
                 raise ValueError(f"{name}: out overlaps {what} without being {what}")
-        note_raw_write()
-        if not out.is_inference():
-            torch.autograd.graph.increment_version(out)      # a graph that saved it must not read the new values
+        _note_written(out)
     if norm_scale.data_ptr() % 16:
         norm_scale = norm_scale.clone()
     nb = m // rows
@@ -783,7 +788,7 @@ def orthogonal_step_(param: torch.Tensor, grad: torch.Tensor, moment: torch.Tens
     _launch(dev, _lib.load().k2q_orthogonal_step, "k2q_orthogonal_step", param.data_ptr(), grad.data_ptr(), moment.data_ptr(),
             C.byref(pl), layout.table.data_ptr(), float(lr), float(momentum), bool(nesterov), float(weight_decay),
             _STEP_SCALES[scale], int(steps), float(eps), float(max_norm), _opt_ptr(normsq), bool(zero_grad), ws.data_ptr(), pl.workspace_bytes)
-    note_raw_write()
+    _note_written(param, moment, *((grad,) if zero_grad else ()))
 
 
 def orthogonalize(u: torch.Tensor, layout: MatrixLayout, steps: int = 5, eps: float = 1e-7,
@@ -800,7 +805,7 @@ def orthogonalize(u: torch.Tensor, layout: MatrixLayout, steps: int = 5, eps: fl
     ws = torch.empty(pl.workspace_bytes // 4, dtype=torch.float32, device=dev)
     _launch(dev, _lib.load().k2q_orthogonalize, "k2q_orthogonalize", u.data_ptr(), out.data_ptr(), C.byref(pl),
             layout.table.data_ptr(), int(steps), float(eps), ws.data_ptr(), pl.workspace_bytes)
-    note_raw_write()
+    _note_written(out)
     return out
 
 

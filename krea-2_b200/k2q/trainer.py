@@ -132,6 +132,8 @@ class FusedOrthogonalStep(_FlatAdapterStep):
                              momentum=self.momentum, nesterov=self.nesterov, weight_decay=self.weight_decay, scale=self.scale,
                              steps=self.steps, eps=self.eps, max_norm=float(self.max_grad_norm or 0.0),
                              normsq=self.normsq if clip else None, zero_grad=True)
+        # the modules' tensors share the buffer's memory, not its version
+        torch.autograd.graph.increment_version([p for b in self.buckets.buckets for p in b["params"]])
         self._rearm()
 
     def state_dict(self) -> dict:
