@@ -479,7 +479,7 @@ def _check_out(name, out, m, n, dev):
         raise RuntimeError(f"{name}: out lives on {out.device}, the operands on {dev}")
     if out.stride(1) != 1 or (m > 1 and out.stride(0) < n):
         raise ValueError(f"{name}: out needs unit inner stride and a row stride >= {n}")
-    note_raw_write()
+    _note_written(out)
 
 
 def _check_lora(name, u, bm, m, n):
