@@ -344,7 +344,8 @@ int k2q_adamw_clip_f32(float* p, float* g, float* m, float* v, int64_t n, float 
  * g is first scaled by min(1, max_norm / (sqrt(*normsq_dev) + 1e-6)) (max_norm <= 0 or normsq_dev NULL: not),
  * and zeroed at the end when zero_grad != 0.  A matrix whose u is zero moves by its weight decay alone; one
  * with a NaN, or whose sum of squares leaves the fp32 range, becomes NaN and leaves the others alone.
- * k2q_orthogonalize gives X of a given u (out may be u).  All sums are formed in a fixed order.
+ * k2q_orthogonalize gives X of a given u (out may be u).  eps is finite and not negative.  All sums are formed in a fixed
+ * order.
  *   k2q_matrices_plan    host only: sizes of the table and the workspace for these shapes
  *   k2q_matrices_table   host only: fills table_host (plan.table_bytes); the caller copies it to 16-byte aligned
  *                        device memory once, it depends on the shapes alone and is only read

@@ -445,7 +445,11 @@ __global__ void __launch_bounds__(WARPS * 32) poly_kernel(const StepParams a) {
     double tr = 0.0;
     for (int i = threadIdx.x; i < t.s; i += 32) tr += g[i * pitch + i];
     for (int o = 16; o > 0; o >>= 1) tr += __shfl_xor_sync(0xffffffffu, tr, o);
-    if (threadIdx.x == 0) inv = 1.0 / (sqrt(tr) + static_cast<double>(a.eps));
+    if (threadIdx.x == 0) {
+      // u of norm zero (squares below 1e-30^2 are zero in fp32 too): any factor serves that P keeps finite in fp32
+      const double norm = sqrt(tr) + static_cast<double>(a.eps);
+      inv = norm < 1e-30 ? 1e30 : 1.0 / norm;
+    }
   }
   __syncthreads();
   const double f = inv;
@@ -680,6 +684,7 @@ int run_steps(const char* name, const k2q_matrices* pl, const void* table, StepP
   if (int rc = check_device_arch()) return rc;
   if (!pl || !table || off16(table) || pl->count <= 0) return fail(K2Q_EINVAL, "%s: no matrix table", name);
   if (!ws || off16(ws) || ws_bytes < pl->workspace_bytes) return fail(K2Q_EINVAL, "%s: workspace too small", name);
+  if (!(a.eps >= 0.f) || a.eps > 3.4e38f) return fail(K2Q_EINVAL, "%s: eps must be a finite number, not negative", name);
   if (a.steps < 0 || a.steps > 10) return fail(K2Q_EINVAL, "%s: steps %d not in [0,10]", name, a.steps);
   a.mats = static_cast<const Mat*>(table);
   a.tiles = reinterpret_cast<const Tile*>(a.mats + pl->count);
