@@ -20,7 +20,10 @@
 // meanwhile by asynchronous copies into a raw area where every thread reads back only what it copied itself.
 // The S x S iteration is in 64 bits, on the fp64 tensor instructions (8 x 8 tiles of the upper triangle): P's entries reach a^steps, so what G_0 loses to rounding comes back up to
 // that much larger in the weak directions.  G_0's products are summed in fp32 by each thread over its share of a piece
-// (a few hundred terms), over threads in fp32, over pieces in 64 bits.  All sums run in a fixed order.
+// (10 terms of each sub-block at rank 32, 32 at rank 64, of the up to 32 sub-blocks of a piece: 1024 at most), over threads
+// in fp32, over pieces in 64 bits.  All sums run in a fixed order.  Relative error of X_5 against 64 bits on gradients with one
+// strong direction: 0.7e-6 with one sub-block to a piece (rank 57), 3e-6 with 7 to 13 (rank 32, 64), 5e-6 with 30 (rank 64); the
+// iteration on the data itself in fp32 has 1e-6.
 // Measured on a B200 (copy bandwidth 6.55 TB/s), 224 adapter matrices, 58.7 M elements:
 //   rank 32   353 us in all (launched one by one: gram 139, poly 25, apply 200).  20 B per element, which a single pass
 //             could not do without, would take 179 us, the 28 B of two passes 251
