@@ -155,7 +155,7 @@ int k2q_gate_residual(const void* x_or_null, int64_t ldx, const void* y, int64_t
  * between the loads and the stores is fp32; the norm reads the stream as it is kept (bf16).  Row strides are
  * multiples of 8 elements, bases 16-byte aligned, K <= 16384.
  *   quant  K a multiple of 128: h rotated and quantised like k2q_fwht_quant_act_i8 (xq [M, K], sx [M]); stream
- *          may be x itself (same pointer and stride) or y itself, but must not overlap them otherwise
+ *          may be x itself (same pointer and stride) or y itself, but must not overlap them otherwise, nor the vectors
  *   fwd    K a multiple of 8: dense h [M, ldh] and rstd [M]; the same rule for stream; h overlaps nothing
  *   bwd    from dstream, dh (either NULL: zero), the kept stream, rstd:  n = stream * rstd,
  *          g = dh (1 + norm_scale)(1 + mod_scale_b),  d = dstream + rstd (g - n mean(g n))

@@ -320,6 +320,12 @@ def _row_stride(t2: torch.Tensor) -> int:
     return t2.stride(0) if t2.shape[0] > 1 else t2.shape[1]
 
 
+def _spans_meet(address: int, nbytes: int, t: torch.Tensor) -> bool:
+    """Whether ``t``, from its first to its last element, meets ``nbytes`` bytes at ``address``."""
+    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1
+    return t.numel() > 0 and t.data_ptr() < address + nbytes and address < t.data_ptr() + last * t.element_size()
+
+
 def _check_residual(name, x, y, norm_scale, k):
     if x.dtype != torch.bfloat16 or y.dtype != torch.bfloat16 or x.dim() < 2 or x.shape != y.shape:
         raise ValueError(f"{name}: x and y must be bf16 tensors [..., L, K] of one shape")
@@ -366,6 +372,9 @@ def residual_norm_quant(x: torch.Tensor, y: torch.Tensor, norm_scale: torch.Tens
         for what, p, ld in (("x", xp, ldx), ("y", yp, ldy)):
             if op < p + ((m - 1) * ld + k) * 2 and p < op + ((m - 1) * ldo + k) * 2 and not (op == p and ldo == ld):
                 raise ValueError(f"{name}: out overlaps {what} without being {what}")
+        for what, t in (("norm_scale", norm_scale), ("gate", gate), ("mod_scale", mod_scale), ("mod_shift", mod_shift)):
+            if t is not None and _spans_meet(op, ((m - 1) * ldo + k) * 2, t):
+                raise ValueError(f"{name}: out overlaps {what}, which every row of a sample reads")
         _note_written(out)
     if norm_scale.data_ptr() % 16:
         norm_scale = norm_scale.clone()
