@@ -222,7 +222,8 @@ int k2q_gemm_w4a8(const int8_t* xq, const uint8_t* wq4, const void* sw4_bf16, in
 
 /* K4 for a few token rows (M <= 32: the timestep MLP and projection, mmdit.py:360-375, short prompts): the
  * same operands, epilogue and BITS as k2q_gemm_w4a8 -- exact integer group sums, scales folded in ascending
- * order of the groups -- in a kernel bound by reading the codes once.  K <= 131072; xq, wq4 and sw4
+ * order of the groups -- in a kernel that reads the codes once (that bounds it for wide products and up to eight rows;
+ * beyond, and with few channels, arithmetic and latency do).  K <= 131072; xq, wq4 and sw4
  * 16-byte aligned.  No waits on other threads' progress, hence no status block.       */
 int k2q_gemv_w4a8(const int8_t* xq, const uint8_t* wq4, const void* sw4_bf16, int64_t M, int64_t N, int64_t K,
                   const k2q_epilogue* ep, void* y_bf16, int64_t ldy, void* stream);

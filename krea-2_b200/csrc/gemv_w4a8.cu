@@ -5,7 +5,7 @@
 //
 // The group sums are exact integers and the scales enter in ascending order of the groups, one fused
 // multiply-add each: the operations of the large W4A8 product on every element, so both give the same bits.
-// Bound by reading the codes once: N*K/2 bytes.
+// Cannot do with less than reading the codes once, N*K/2 bytes, and is bound by that for wide products and up to eight rows.
 //
 // A warp owns 8 or 16 channels and folds its groups in registers.  A group of eight channels is four m16n8k32 int8 MMAs
 // per 16 tokens, the tokens as rows (dp4a reaches a quarter of their rate, and needs the codes as bytes as well).  The

@@ -18,20 +18,21 @@
 // is the contiguous one in memory (gram of a wide matrix, apply of a tall one) the sub-block stays as it is
 // ("natural"), otherwise neighbouring rows are interleaved on the way in ("paired").  The next sub-block travels
 // meanwhile by asynchronous copies into a raw area where every thread reads back only what it copied itself.
-// The S x S iteration is in 64 bits, on the fp64 tensor instructions (8 x 8 tiles of the upper triangle): P's entries reach a^steps, so what G_0 loses to rounding comes back up to
-// that much larger in the weak directions.  G_0's products are summed in fp32 by each thread over its share of a piece
-// (10 terms of each sub-block at rank 32, 32 at rank 64, of the up to 32 sub-blocks of a piece: 1024 at most), over threads
-// in fp32, over pieces in 64 bits.  All sums run in a fixed order.  Relative error of X_5 against 64 bits on gradients with one
-// strong direction: 0.7e-6 with one sub-block to a piece (rank 57), 3e-6 with 7 to 13 (rank 32, 64), 5e-6 with 30 (rank 64); the
-// iteration on the data itself in fp32 has 1e-6.
+// The S x S iteration is in 64 bits, on the fp64 tensor instructions (8 x 8 tiles of the upper triangle): P's entries reach
+// a^steps, so what G_0 loses to rounding comes back up to that much larger in the weak directions.  G_0's products are summed
+// in fp32 by each thread over its share of a piece (10 terms of each sub-block at rank 32, 32 at rank 64, of the up to 32
+// sub-blocks of a piece: 1024 at most), over threads in fp32, over pieces in 64 bits.  All sums run in a fixed order.
+// Relative error of X_5 against 64 bits on gradients with one strong direction: 0.7e-6 with one sub-block to a piece (rank
+// 57), 3e-6 with 7 to 13 (rank 32, 64), 5e-6 with 30 (rank 64); the iteration on the data itself in fp32 has 1e-6.
 // Measured on a B200 (copy bandwidth 6.55 TB/s), 224 adapter matrices, 58.7 M elements:
 //   rank 32   353 us in all (launched one by one: gram 139, poly 25, apply 200).  20 B per element, which a single pass
 //             could not do without, would take 179 us, the 28 B of two passes 251
 //   rank 16   144 us for 22 M elements (67 at 20 B each)      rank 64, half the matrices, 58.7 M elements   568 us
-// Counters of gram / apply at rank 32: shared memory 61 / 55 % of its rate, issue 57 / 52 %, DRAM 54 / 49 %, fp32 pipe 27 / 24 %,
-// at 21 / 15 warps per SM: latency between units that are each half busy.  Taking apply's pieces backwards, to find the
-// last of gram's in L2, saved 5 % of its reads and 0.4 % of the time, and is not done.  At rank 64: shared memory 63 / 63 %,
-// DRAM 29 / 32 %, fp32 pipe 28 / 28 %; gram waits most at its barriers.  The iteration takes 52 us there, on one SM per matrix.
+// Counters of gram / apply at rank 32: shared-memory wavefronts 71 / 65 % of the pipe's, issue 59 / 54 %, DRAM 58 / 55 %, fp32
+// pipe 38 / 37 %, at 22 / 15 warps per SM: shared memory is the busiest and no unit is full.  Taking apply's pieces
+// backwards, to find the last of gram's in L2, saved 5 % of its reads and 0.4 % of the time, and is not done.  At rank 64:
+// 73 / 71 %, issue 50 / 53 %, DRAM 36 / 37 %, fp32 pipe 42 / 46 %; gram waits most at its barriers.  The iteration takes
+// 52 us there, on one SM per matrix.  apply spills 8 bytes of a thread at 128 registers.
 #include "k2q_common.cuh"
 
 namespace k2q {

@@ -13,14 +13,16 @@
 //
 // Everything between the loads and the stores is fp32; the stream is rounded to bf16 once, where it is
 // kept, and the norm reads the rounded values, so that the backward sees the same numbers.  b = row /
-// rows_per_batch.  They move 7, 8 and 10 (12 with the sums) bytes per element; the forward and the backward without sums are held by HBM, the others by what follows.  A row is worked on by
-// one CTA (its two reductions are CTA-wide); a CTA takes consecutive rows of one sample, so that the sample's vectors are
-// read from L2 once per CTA and not once per row, and there are exactly as many CTAs as the SMs hold at once.  The
-// quantising kernel is held to 96 registers, so that three CTAs of 192 threads fit (at 124, two did, in 1.5 waves): that,
-// with the shift and gate left as bf16 and the rotation's factor folded into the row scale, took it from 237 to 181 us.
+// rows_per_batch.  They move 7, 8 and 10 (12 with the sums) bytes per element; the forward and the backward without sums
+// are held by HBM, the others by what follows.  A row is worked on by one CTA (its two reductions are CTA-wide); a CTA takes
+// consecutive rows of one sample, so that the sample's vectors are read from L2 once per CTA and not once per row, and there
+// are exactly as many CTAs as the SMs hold at once.  The quantising kernel is held to 96 registers (up to 16 bytes of a
+// thread spill), so that three CTAs of 192 threads fit (at 124, two did, in 1.5 waves): that, with the shift and gate left
+// as bf16 and the rotation's factor folded into the row scale, took it from 237 to 181 us.
 // Measured on a B200 (copy bandwidth 6.55 TB/s), 16896 rows of 6144, gate and modulation:
 //   quantising  137 us = 5.3 TB/s (0.81)      forward  138 us = 6.0 TB/s (0.92)
 //   backward    187 us = 5.55 TB/s (0.85)     with every sum  280 us = 4.45 TB/s (0.68)
+// (the chain of the two single kernels, cold: quantising 440 us, forward 248, forward and backward 630 against 336 here).
 // The quantising kernel executes 22 instructions per element, 4 warps to an SM quarter, and issues in 49 % of the cycles;
 // the largest stall is on shuffles and shared memory (the sample's vectors).  The backward with sums keeps them in shared
 // memory above 4096 columns: one CTA of 12 warps per SM at 128 registers, 53 % of the shared-memory rate, 39 % issue, most

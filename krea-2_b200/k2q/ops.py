@@ -571,14 +571,18 @@ GEMV_MAX_K = 131072
 # Rows that gemm_w4a8 hands to it.  Measured on a B200 with weights from DRAM, few-row kernel against the large
 # product's: 16 rows 27.0 / 68.8 us at 36864 x 6144, 11.8 / 27.6 at 6144 x 6144, 18.4 / 37.0 at 16384 x 6144, 3.8 / 5.8
 # at 6144 x 256; 32 rows 43.3 / 52.3, 20.7 / 27.2, 29.7 / 28.0, 5.3 / 5.8 -- between the two the large product's tiles
-# start to fill the SMs, and the few-row kernel's token reads to cost as much as the codes.
+# start to fill the SMs, and the few-row kernel's token reads to cost as much as the codes.  Over 16 to 36864 channels,
+# contractions of 128 to 16384, 1, 8 and 16 rows and ranks 0, 16 and 32 the few-row kernel was never the slower one; with an
+# adapter term it takes 0.2 to 0.6 of the large product's time (36864 x 6144, 16 rows, rank 32: 64 us against 119).
 GEMV_BEST_ROWS = 16
 
 
 def gemv_w4a8(xq, sx, wq4, sw4, bias=None, u=None, bm=None, lora_scale: float = 0.0, act=None,
               out: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`gemm_w4a8` for up to ``GEMV_ROWS`` token rows (one timestep vector per image, a short prompt): the
-    same operands and the same bits, from a kernel that is bound by reading the 4-bit codes once."""
+    same operands and the same bits, from a kernel that reads the 4-bit codes once.  That bounds it for wide products and
+    up to eight rows; beyond, and with few channels, arithmetic and latency do (see ``GEMV_BEST_ROWS`` for where the
+    large product catches up)."""
     name = "gemv_w4a8"
     dev = _one_device(xq, sx, wq4, sw4, bias, u, bm)
     m, n, k = _check_w4a8(name, xq, sx, wq4, sw4, bias, u, bm)
